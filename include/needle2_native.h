@@ -294,6 +294,61 @@ int needle2_gpu_kv_import(void *kv, int layer, int seq, const int8_t *k, const i
 int needle2_gpu_kv_export(void *kv, int layer, int seq, int8_t *k, int8_t *v, float *k_scales, float *v_scales,
                           int first_slot, int count);
 
+/* ---- long contexts over the int8 KV cache -----------------------------------
+ * The reference attends one sequence's window through a slot list
+ * (needle2/csrc/engine.cpp:898-911) and neither shares a prefix between
+ * sequences nor drops slots; these serve a batch. heads: a multiple of kvheads,
+ * 1 to 16 query heads per kv head. Nothing is read on the host, so every call
+ * can be captured once it has run with the same sizes (its scratch belongs to
+ * the handle, is never moved while the handle lives, and is not for two calls
+ * at once). The handle must have been made on the current device. All return
+ * 0 / -1 (message in needle2_gpu_error); a refused call does nothing. */
+
+/* Attention of `count` consecutive new tokens per sequence over a window with
+ * pinned first positions. d_q, d_out: device fp32 [seqs][count][heads][head_dim].
+ * Token i of sequence s is at position d_positions[s] + i (device; + count
+ * stays below 2^31). Position p lies in slot p for p < sinks, then in slot
+ * sinks + (p - sinks) % (capacity - sinks). First stores the tokens' rows
+ * (d_new_k, d_new_v [seqs][count][kvheads][head_dim] fp32; both NULL: they are
+ * stored already), then token i attends every position up to its own that is
+ * below sinks or among the last `window`. A token at a negative position (left
+ * padding, an idle sequence) is not stored and its output is zero. Needs
+ * sinks + window + count - 1 <= capacity, at most 2^26 query rows. */
+int needle2_gpu_attention_window(void *kv, int layer, const float *d_q, float *d_out, int heads, int count,
+                                 const int *d_positions, int sinks, int window, const float *d_new_k,
+                                 const float *d_new_v, void *stream);
+/* One decode step of sequences that share a prefix: every query attends slots
+ * [0, prefix_length) of sequence prefix_seq of `prefix` (another cache of the
+ * same kvheads and head_dim; the same layer) and its own slots [0, n),
+ * n = d_lengths[s] (device; NULL: length), at most `length`. The prefix's rows
+ * are read once for the batch. d_new_k, d_new_v ([seqs][kvheads][head_dim]
+ * fp32, both or none): the step's token, first stored in slot n - 1. */
+int needle2_gpu_attention_shared(void *kv, int layer, void *prefix, int prefix_seq, int prefix_length, const float *d_q,
+                                 float *d_out, int heads, int length, const int *d_lengths, const float *d_new_k,
+                                 const float *d_new_v, void *stream);
+/* One decode step over slots [0, n) as above that also adds to
+ * d_weights[s][kvhead][slot] (device fp32 [seqs][kvheads][capacity]) the slot's
+ * softmax weights, summed over the kv head's query heads; entries from n on are
+ * left as they are. A head without a softmax (a non-finite query) adds nothing. */
+int needle2_gpu_attention_weights(void *kv, int layer, const float *d_q, float *d_out, float *d_weights, int heads,
+                                  int length, const int *d_lengths, const float *d_new_k, const float *d_new_v,
+                                  void *stream);
+/* Cuts every sequence of a layer to `keep` slots. With n = d_lengths[s]
+ * (clamped to [0, capacity]) and n > keep, each kv head keeps slots
+ * [0, sinks), [n - recent, n) and, of those between, the
+ * keep - sinks - recent with the largest d_weights (of equal ones the lower
+ * slots; NaN ranks lowest); with n <= keep all of them. Kept rows and weights
+ * move to slots 0, 1, .. in their order; rows behind them keep what they held.
+ * d_new_weights (may be d_weights, else disjoint) gets the kept weights and
+ * zeros up to the capacity, d_new_lengths[s] (may be d_lengths) min(n, keep),
+ * d_kept ([seqs][kvheads][keep], nullable) the old slots, -1 past the last.
+ * sinks + recent <= keep <= capacity, keep >= 1. */
+int needle2_gpu_kv_evict(void *kv, int layer, const float *d_weights, const int *d_lengths, int keep, int sinks,
+                         int recent, float *d_new_weights, int *d_new_lengths, int *d_kept, void *stream);
+/* Device addresses of a layer's rows: codes [seqs][kvheads][capacity][head_dim]
+ * and fp32 scales [seqs][kvheads][capacity], valid while the handle lives. */
+int needle2_gpu_kv_layer(void *kv, int layer, int8_t **d_k, int8_t **d_v, float **d_k_scales, float **d_v_scales);
+
 #ifdef __cplusplus
 }
 #endif

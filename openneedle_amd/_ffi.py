@@ -106,6 +106,11 @@ SIGNATURES: dict[str, tuple] = {
     "needle2_gpu_attention_chained": (i32, [vp, i32, vp, vp, i32, i32, vp, vp, i32, vp, vp, vp, vp, vp]),
     "needle2_gpu_kv_import": (i32, [vp, i32, i32, vp, vp, vp, vp, i32, i32]),
     "needle2_gpu_kv_export": (i32, [vp, i32, i32, vp, vp, vp, vp, i32, i32]),
+    "needle2_gpu_attention_window": (i32, [vp, i32, vp, vp, i32, i32, vp, i32, i32, vp, vp, vp]),
+    "needle2_gpu_attention_shared": (i32, [vp, i32, vp, i32, i32, vp, vp, i32, i32, vp, vp, vp, vp]),
+    "needle2_gpu_attention_weights": (i32, [vp, i32, vp, vp, vp, i32, i32, vp, vp, vp, vp]),
+    "needle2_gpu_kv_evict": (i32, [vp, i32, vp, vp, i32, i32, i32, vp, vp, vp, vp]),
+    "needle2_gpu_kv_layer": (i32, [vp, i32, vp, vp, vp, vp]),
 }
 
 

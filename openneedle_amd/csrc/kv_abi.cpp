@@ -6,40 +6,13 @@
 // This library exposes the same arithmetic as a device-resident cache for
 // many sequences at once: store quantizes new K/V rows, attention runs one
 // decode step for every sequence of one layer.
-#include "abi_internal.h"
 #include "attn.h"
+#include "kv.h"
 
 #include <algorithm>
 #include <cmath>
-#include <memory>
-#include <vector>
 
 namespace nd {
-
-struct KvHandle {
-    int layers = 0, capacity = 0, kvheads = 0, head_dim = 0, seqs = 0;
-    DevBuf<int8_t> k8, v8;
-    DevBuf<float> ks, vs;
-    DevBuf<float> part;
-    DevBuf<int> first;    // per-sequence first slot of a store
-    HostBuf<int> hfirst;  // pinned staging for `first`
-    hipEvent_t first_copied = nullptr;
-
-    size_t layer_codes() const { return size_t(seqs) * kvheads * capacity * head_dim; }
-    size_t layer_scales() const { return size_t(seqs) * kvheads * capacity; }
-    ~KvHandle() {
-        if (first_copied) (void)hipEventDestroy(first_copied);
-    }
-};
-
-static KvHandle *kv_of(void *h) {
-    ND_CHECK(h != nullptr, "null KV cache handle");
-    return static_cast<KvHandle *>(h);
-}
-
-static void check_layer(const KvHandle &kv, int layer) {
-    ND_CHECK(layer >= 0 && layer < kv.layers, "KV cache: layer out of range");
-}
 
 // Splits of the slot range: enough (sequence, kv head, split) blocks for two
 // per CU, never a split shorter than one 256-slot tile. With that many
@@ -81,6 +54,7 @@ void *needle2_gpu_kv_create(int layers, int capacity, int kvheads, int head_dim,
             h->kvheads = kvheads;
             h->head_dim = head_dim;
             h->seqs = seqs;
+            ND_HIP(hipGetDevice(&h->device));
             const size_t nc = h->layer_codes() * layers, ns = h->layer_scales() * layers;
             h->k8.reserve(nc);
             h->v8.reserve(nc);

@@ -10,11 +10,13 @@ reference's layout, ``[slots][kvheads][head_dim]`` int8 and
 """
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 
 from . import _ffi
 from ._ffi import GpuError, addr, check
-from .device import stream_ptr
+from .device import DeviceView, stream_ptr
 
 
 class KVCache:
@@ -64,6 +66,60 @@ class KVCache:
                                                           addr(nk), addr(nv), addr(ns),
                                                           next.ptr if next is not None else None,
                                                           stream_ptr(stream)), "attention")
+
+    def attention_window(self, layer: int, d_q, d_out, heads: int, count: int, d_positions, sinks: int, window: int,
+                         stream=None, new=None) -> None:
+        """``count`` consecutive tokens per sequence over a window with pinned first positions: device q / out fp32
+        ``[seqs][count][heads][head_dim]``. Token ``i`` of sequence ``s`` is at position ``d_positions[s] + i`` and
+        attends the positions up to its own that are below ``sinks`` or among the last ``window``. Position ``p`` lies
+        in slot ``p`` for ``p < sinks``, then in slot ``sinks + (p - sinks) % (capacity - sinks)``; ``new``: (device k,
+        device v) ``[seqs][count][kvheads][head_dim]`` of these tokens, stored there first. A negative position is a
+        padded token: not stored, output zero. Needs ``sinks + window + count - 1 <= capacity``."""
+        nk, nv = new if new is not None else (None, None)
+        check(self._lib.needle2_gpu_attention_window(self.ptr, layer, addr(d_q), addr(d_out), int(heads), int(count),
+                                                     addr(d_positions), int(sinks), int(window), addr(nk), addr(nv),
+                                                     stream_ptr(stream)), "window attention")
+
+    def attention_shared(self, layer: int, prefix: "KVCache", prefix_length: int, d_q, d_out, heads: int, length: int,
+                         d_lengths=None, prefix_seq: int = 0, stream=None, new=None) -> None:
+        """One decode step of sequences behind one prefix: every sequence attends the first ``prefix_length`` slots of
+        sequence ``prefix_seq`` of ``prefix`` (another cache, read once for the batch) and its own first
+        ``d_lengths[s]`` (default and at most ``length``) slots. ``new``: (device k, device v)
+        ``[seqs][kvheads][head_dim]`` of the step's token, stored first in each sequence's last attended slot."""
+        nk, nv = new if new is not None else (None, None)
+        check(self._lib.needle2_gpu_attention_shared(self.ptr, layer, prefix.ptr, int(prefix_seq), int(prefix_length),
+                                                     addr(d_q), addr(d_out), int(heads), int(length), addr(d_lengths),
+                                                     addr(nk), addr(nv), stream_ptr(stream)), "shared-prefix attention")
+
+    def attention_weights(self, layer: int, d_q, d_out, d_weights, heads: int, length: int, d_lengths=None, stream=None,
+                          new=None) -> None:
+        """One decode step over every sequence's first ``d_lengths[s]`` (default and at most ``length``) slots that adds
+        each slot's softmax weights, summed over the kv head's query heads, to device fp32 ``d_weights``
+        ``[seqs][kvheads][capacity]``. ``new`` as for :meth:`attention_shared`."""
+        nk, nv = new if new is not None else (None, None)
+        check(self._lib.needle2_gpu_attention_weights(self.ptr, layer, addr(d_q), addr(d_out), addr(d_weights), int(heads),
+                                                      int(length), addr(d_lengths), addr(nk), addr(nv),
+                                                      stream_ptr(stream)), "weight-recording attention")
+
+    def evict(self, layer: int, d_weights, d_lengths, keep: int, sinks: int, recent: int, d_new_weights, d_new_lengths,
+              d_kept=None, stream=None) -> None:
+        """Cut every sequence of ``layer`` with more than ``keep`` slots: per kv head the first ``sinks``, the last
+        ``recent`` and, of those between, the ones with the largest ``d_weights`` (of equal ones the lower slots) move to
+        slots ``0 .. keep - 1`` in their order. ``d_new_weights`` (may be ``d_weights``): the kept slots' weights, then
+        zeros; ``d_new_lengths`` (may be ``d_lengths``): the slots left; ``d_kept``: int32 ``[seqs][kvheads][keep]``, the
+        old slots (-1 past the last). Capturable."""
+        check(self._lib.needle2_gpu_kv_evict(self.ptr, layer, addr(d_weights), addr(d_lengths), int(keep), int(sinks),
+                                             int(recent), addr(d_new_weights), addr(d_new_lengths), addr(d_kept),
+                                             stream_ptr(stream)), "eviction")
+
+    def device_rows(self, layer: int):
+        """(k codes, v codes, k scales, v scales) of one layer as device memory of this cache, not copied: int8
+        ``[seqs][kvheads][capacity][head_dim]`` and fp32 ``[seqs][kvheads][capacity]``."""
+        at = [ctypes.c_void_p() for _ in range(4)]
+        check(self._lib.needle2_gpu_kv_layer(self.ptr, layer, *(ctypes.byref(a) for a in at)), "KV layer")
+        rows = self.seqs * self.kvheads * self.capacity
+        sizes = (rows * self.head_dim, rows * self.head_dim, rows * 4, rows * 4)
+        return tuple(DeviceView(self, a.value - self.ptr, n) for a, n in zip(at, sizes))
 
     def load(self, layer: int, seq: int, k, v, ks, vs, first_slot: int = 0) -> None:
         """Copy host int8 rows and fp32 scales (reference layout) into one sequence of the cache."""

@@ -177,9 +177,10 @@ def prepare(case, seed):
 
 
 class _Address:
-    """Device memory as torch takes it."""
+    """Device memory as torch takes it; the tensor keeps this object, which keeps the cache."""
 
     def __init__(self, at, kind, shape):
+        self.at = at
         self.__cuda_array_interface__ = dict(data=(at.ptr, False), typestr=kind, shape=shape, version=2)
 
 

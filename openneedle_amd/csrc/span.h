@@ -58,6 +58,8 @@ constexpr int kSpanRows = 16;      // query rows of a block
 
 void launch_span_store(const SpanStoreArgs &a, hipStream_t s);
 void launch_span(const SpanArgs &a, int head_dim, hipStream_t s);
+// the same in blocks of 32 * waves query rows (waves 1 to 4)
+void launch_span_wide(const SpanArgs &a, int head_dim, int waves, hipStream_t s);
 // out rows from all their records
 void launch_span_join(const SpanArgs &a, int head_dim, hipStream_t s);
 void launch_span_record(const SpanRecordArgs &a, int head_dim, hipStream_t s);

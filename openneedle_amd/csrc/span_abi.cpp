@@ -41,15 +41,41 @@ static SpanArgs span_args(KvHandle &kv, const SpanCache &c, const float *d_q, fl
     return a;
 }
 
-// Pieces of a unit's `tiles` tiles: two blocks per compute unit, of whole rounds of a block's four waves.
-static void cut(SpanArgs &a, int tiles) {
-    const int64_t row_tiles = (int64_t(a.count) * a.group + kSpanRows - 1) / kSpanRows;
-    const int64_t blocks = std::max<int64_t>(1, row_tiles * a.kvheads * a.units);
-    const int rounds = std::max(1, (tiles + 3) / 4);
-    const int want = static_cast<int>(std::min<int64_t>(rounds, (2 * device_cus() + blocks - 1) / blocks));
+// How a launch is cut: `waves` 0 for the 16-row kernel, else the wide kernel's row groups of 32 per block.
+struct SpanPlan {
+    int waves = 0;
+};
+
+// Pieces of a unit's keys (at most `keys` in `runs` runs): two blocks per compute unit, of whole rounds of a block.
+static SpanPlan cut(SpanArgs &a, int keys, int runs) {
+    const int64_t rows = int64_t(a.count) * a.group;
+    SpanPlan p;
+    if (rows > kSpanRows) {
+        double best = 0;
+        for (int w = 4; w >= 1; --w) {
+            const double cost = double((rows + 32 * w - 1) / (32 * w)) * (w + 0.6);
+            if (!p.waves || cost < best) {
+                best = cost;
+                p.waves = w;
+            }
+        }
+    }
+    const int block_rows = p.waves ? 32 * p.waves : kSpanRows;
+    const int64_t blocks = std::max<int64_t>(1, (rows + block_rows - 1) / block_rows * a.kvheads * a.units);
+    const int round = p.waves ? 1 : 4;  // tiles of a block's round
+    const int tiles = (p.waves ? wide_tiles(keys) : span_tiles(keys)) + runs - 1;
+    const int rounds = std::max(1, (tiles + round - 1) / round);
+    const int target = 2 * device_cus();
+    const int want = static_cast<int>(std::min<int64_t>(rounds, std::max<int64_t>(1, target / blocks)));
     const int per_rounds = (rounds + want - 1) / want;
-    a.per = 4 * per_rounds;
+    a.per = round * per_rounds;
     a.splits = (rounds + per_rounds - 1) / per_rounds;
+    return p;
+}
+
+static void launch(const SpanArgs &a, const SpanPlan &p, int head_dim, hipStream_t s) {
+    if (p.waves) launch_span_wide(a, head_dim, p.waves, s);
+    else launch_span(a, head_dim, s);
 }
 
 // Room for the records of `rows` rows.
@@ -85,9 +111,10 @@ int needle2_gpu_attention_window(void *h, int layer, const float *d_q, float *d_
         a.positions = d_positions;
         a.sinks = sinks;
         a.window = window;
-        // keys of a row tile: its tokens' windows, and one tile more for the second run
-        const int tokens = std::min(count, (kSpanRows + a.group - 1) / a.group + 1);
-        cut(a, span_tiles(sinks + window + tokens - 1) + 1);
+        // keys of a block: its tokens' windows
+        const int most = int64_t(count) * a.group <= kSpanRows ? kSpanRows : 128;
+        const int tokens = std::min(count, (most + a.group - 1) / a.group + 1);
+        const SpanPlan plan = cut(a, sinks + window + tokens - 1, 2);
         a.splits_total = a.splits;
         if (a.splits_total > 1) reserve_records(kv, a, int64_t(kv.seqs) * count * heads);
         if (d_new_k && count == 1) {
@@ -106,7 +133,7 @@ int needle2_gpu_attention_window(void *h, int layer, const float *d_q, float *d_
             st.sinks = sinks;
             launch_span_store(st, s);
         }
-        launch_span(a, kv.head_dim, s);
+        launch(a, plan, kv.head_dim, s);
         if (a.splits_total > 1) launch_span_join(a, kv.head_dim, s);
     });
 }
@@ -131,10 +158,10 @@ int needle2_gpu_attention_shared(void *h, int layer, void *prefix, int prefix_se
         own.lengths = d_lengths;
         own.new_k = d_new_k;
         own.new_v = d_new_v;
-        cut(own, span_tiles(length));
+        const SpanPlan own_plan = cut(own, length, 1);
         SpanArgs far = span_args(kv, layer_of(pre, layer, prefix_seq), d_q, d_out, 1, heads, kv.seqs);
         far.length = prefix_length;
-        cut(far, span_tiles(prefix_length));
+        const SpanPlan far_plan = cut(far, prefix_length, 1);
         if (prefix_length == 0) far.splits = 0;
         own.split0 = far.splits;
         own.splits_total = far.splits_total = far.splits + own.splits;
@@ -143,8 +170,8 @@ int needle2_gpu_attention_shared(void *h, int layer, void *prefix, int prefix_se
             far.rec_o = own.rec_o;
             far.rec_ml = own.rec_ml;
         }
-        if (prefix_length > 0) launch_span(far, kv.head_dim, s);
-        launch_span(own, kv.head_dim, s);
+        if (prefix_length > 0) launch(far, far_plan, kv.head_dim, s);
+        launch(own, own_plan, kv.head_dim, s);
         if (own.splits_total > 1) launch_span_join(own, kv.head_dim, s);
     });
 }
@@ -165,13 +192,13 @@ int needle2_gpu_attention_weights(void *h, int layer, const float *d_q, float *d
         a.new_k = d_new_k;
         a.new_v = d_new_v;
         const int tiles = span_tiles(length);
-        cut(a, tiles);
+        const SpanPlan plan = cut(a, length, 1);
         a.splits_total = a.splits;
         reserve_records(kv, a, int64_t(kv.seqs) * heads);  // for one piece too: the weights need the final sums
         a.score_stride = std::max(1, tiles) * kSpanTile;
         a.scores = kv.scores.reserve(size_t(kv.seqs) * heads * a.score_stride);
         SpanRecordArgs r{a, d_weights};
-        launch_span(a, kv.head_dim, s);
+        launch(a, plan, kv.head_dim, s);
         launch_span_record(r, kv.head_dim, s);
     });
 }

@@ -52,6 +52,9 @@ ND_BOTH KeyRuns ring_runs(int first, int last, int sinks, int window, int capaci
 
 constexpr int kSpanTile = 64;  // keys of a tile; a tile lies in one run
 
+constexpr int kWideTile = 32;  // where many query rows share them
+
 ND_BOTH int span_tiles(int n) { return (n + kSpanTile - 1) / kSpanTile; }
+ND_BOTH int wide_tiles(int n) { return (n + kWideTile - 1) / kWideTile; }
 
 }  // namespace nd

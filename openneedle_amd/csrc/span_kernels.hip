@@ -9,76 +9,14 @@
 //
 // Both products run on v_mfma_f32_16x16x32_bf16. The codes are bfloat16 numbers as they are; q and p * vs are three
 // bfloat16 terms each (8 + 8 + 8 bits: the fp32 value exactly, at any magnitude), so only the sums round, in fp32.
-#include "span.h"
-#include "wave.h"
+#include "span_dev.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace nd {
 
 namespace {
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ float code(uint32_t w, int c) {
-    return static_cast<float>(static_cast<int8_t>((w >> (8 * c)) & 0xffu));
-}
-
-// bfloat16 pair of the upper halves of two fp32 values (the low half from a).
-__device__ __forceinline__ uint32_t upper_halves(float a, float b) {
-    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
-}
-__device__ __forceinline__ float cut(float x) {
-    return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xFFFF0000u);
-}
-
-struct Terms {
-    u32x4 t[3];  // eight values as three bfloat16 terms, the largest first
-};
-
-// The three terms of values 2 i and 2 i + 1. Exact for finite values: every cut leaves 8 bits less.
-__device__ __forceinline__ void split_pair(float a, float b, uint32_t &t0, uint32_t &t1, uint32_t &t2) {
-    t0 = upper_halves(a, b);
-    a -= cut(a);
-    b -= cut(b);
-    t1 = upper_halves(a, b);
-    a -= cut(a);
-    b -= cut(b);
-    t2 = upper_halves(a, b);
-}
-__device__ __forceinline__ Terms split8(const float (&x)[8]) {
-    uint32_t t[3][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) split_pair(x[2 * i], x[2 * i + 1], t[0][i], t[1][i], t[2][i]);
-    Terms r;
-#pragma unroll
-    for (int k = 0; k < 3; ++k) r.t[k] = u32x4{t[k][0], t[k][1], t[k][2], t[k][3]};
-    return r;
-}
-
-// The same where values may be infinite or NaN: those are their first term alone.
-__device__ __forceinline__ Terms split8_any(const float (&x)[8]) {
-    float y[8];
-    bool odd[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        odd[i] = !(fabsf(x[i]) < INFINITY);
-        y[i] = odd[i] ? 0.0f : x[i];
-    }
-    Terms r = split8(y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = odd[i] ? x[i] : y[i];
-    r.t[0] = u32x4{upper_halves(y[0], y[1]), upper_halves(y[2], y[3]), upper_halves(y[4], y[5]), upper_halves(y[6], y[7])};
-    return r;
-}
-
-// Eight codes of two dwords as bfloat16.
-__device__ __forceinline__ u32x4 widen(uint32_t a, uint32_t b) {
-    return u32x4{upper_halves(code(a, 0), code(a, 1)), upper_halves(code(a, 2), code(a, 3)),
-                 upper_halves(code(b, 0), code(b, 1)), upper_halves(code(b, 2), code(b, 3))};
-}
 
 __device__ __forceinline__ f32x4 mfma(const u32x4 &a, const u32x4 &b, const f32x4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -106,10 +44,6 @@ __device__ __forceinline__ void quantise_row(const float *x, int HD, int lane, i
 __device__ __forceinline__ void store_token(const SpanCache &c, const float *k, const float *v, size_t row, int HD, int lane) {
     quantise_row(k, HD, lane, c.k8 + row * HD, c.ks + row);
     quantise_row(v, HD, lane, c.v8 + row * HD, c.vs + row);
-}
-
-__device__ __forceinline__ int at_position(int first, int i) {
-    return static_cast<int>(static_cast<uint32_t>(first) + static_cast<uint32_t>(i));
 }
 
 // One wave per (sequence, token, kv head).
@@ -435,60 +369,113 @@ __global__ __launch_bounds__(256, 2) void span_kernel(SpanArgs a) {
     }
 }
 
-// The row's maximum and sum over its records (empty ones skipped), by one thread.
-__device__ __forceinline__ float2 join_ml(const float2 *ml, int splits) {
-    float M = -INFINITY, L = 0.0f;
-    for (int s = 0; s < splits; ++s) M = fmaxf(M, ml[s].x);
-    const float base = M == -INFINITY ? 0.0f : M;
-    for (int s = 0; s < splits; ++s) {
-        const float2 v = ml[s];
-        if (v.x == -INFINITY && v.y == 0.0f) continue;
-        L = __builtin_fmaf(__builtin_amdgcn_exp2f(v.x - base), v.y, L);
-    }
-    return make_float2(base, L);
-}
-
-// Output d .. d + 3 of one row from its records, in their order.
-__device__ __forceinline__ void join_row(const SpanArgs &a, int HD, size_t row, int d) {
+// A row's maximum and sum over its records, by one wave; the records' factors 2^(m - maximum) to `factor` if that is set.
+__device__ __forceinline__ float2 join_sums(const SpanArgs &a, size_t row, int lane, float *factor) {
     const float2 *ml = a.rec_ml + row * a.splits_total;
-    const float2 all = join_ml(ml, a.splits_total);
-    float o[4] = {0, 0, 0, 0};
-    for (int s = 0; s < a.splits_total; ++s) {
+    float2 mine = make_float2(-INFINITY, 0.0f);  // of this lane's first record: most rows have no second
+    float M = -INFINITY;
+    for (int s = lane; s < a.splits_total; s += 64) {
         const float2 v = ml[s];
-        if (v.x == -INFINITY && v.y == 0.0f) continue;
-        const float f = __builtin_amdgcn_exp2f(v.x - all.x);
-        const float4 p = *reinterpret_cast<const float4 *>(a.rec_o + (row * a.splits_total + s) * HD + d);
-        o[0] = __builtin_fmaf(f, p.x, o[0]);
-        o[1] = __builtin_fmaf(f, p.y, o[1]);
-        o[2] = __builtin_fmaf(f, p.z, o[2]);
-        o[3] = __builtin_fmaf(f, p.w, o[3]);
+        if (s == lane) mine = v;
+        M = fmaxf(M, v.x);
     }
-    const float inv = 1.0f / all.y;
-    *reinterpret_cast<float4 *>(a.out + row * HD + d) =
-        all.y > 0 ? make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv) : make_float4(0, 0, 0, 0);
+    M = wave_max(M, lane);
+    const float base = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f;
+    for (int s = lane; s < a.splits_total; s += 64) {
+        const float2 v = s == lane ? mine : ml[s];
+        const bool empty = v.x == -INFINITY && v.y == 0.0f;
+        const float f = empty ? 0.0f : __builtin_amdgcn_exp2f(v.x - base);
+        if (factor) factor[s] = f;
+        L += empty ? 0.0f : f * v.y;
+    }
+    return make_float2(base, wave_sum(L, lane));
 }
 
-__global__ __launch_bounds__(256) void span_join_kernel(SpanArgs a, int HD, int64_t rows) {
-    const int per = HD / 4;
-    const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / per;
-    if (row < rows) join_row(a, HD, row, threadIdx.x % per * 4);
+// Rows row0 .. row0 + count - 1 from their records, by a block of 256: G groups of HD / 4 lanes share a row's records
+// (every G-th each), whose loads do not wait for each other; 256 / (G * HD / 4) rows at a time. The sums' order depends
+// on the number of records only.
+constexpr int kJoinMax = 1024;  // records of a row
+template <int HD, int G>
+__device__ __forceinline__ void join_rows(const SpanArgs &a, size_t row0, int count) {
+    constexpr int kLanes = HD / 4, kRows = 256 / (G * kLanes);
+    constexpr int kFactors = kRows * (G == 8 ? kJoinMax : G);
+    __shared__ float factor[kFactors];
+    __shared__ float total[kRows];
+    __shared__ __attribute__((aligned(16))) float part[G > 1 ? G : 1][kRows][HD];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int splits = a.splits_total;
+    const int d = t % kLanes * 4, g = t / kLanes % G, r = t / (kLanes * G);
+    for (int i0 = 0; i0 < count; i0 += kRows) {
+        for (int i = wave; i < kRows && i0 + i < count; i += 4) {
+            const float2 all = join_sums(a, row0 + i0 + i, lane, factor + i * splits);
+            if (lane == 0) total[i] = all.y;
+        }
+        __syncthreads();
+        const bool live = i0 + r < count;
+        float4 o = make_float4(0, 0, 0, 0);
+        if (live) {
+            const float *rec = a.rec_o + (row0 + i0 + r) * splits * HD + d;
+#pragma unroll 4
+            for (int s = g; s < splits; s += G) {
+                const float f = factor[r * splits + s];
+                const float4 p = *reinterpret_cast<const float4 *>(rec + static_cast<size_t>(s) * HD);
+                if (f == 0.0f) continue;  // an empty piece, or weights that vanish beside the rest
+                o.x = __builtin_fmaf(f, p.x, o.x);
+                o.y = __builtin_fmaf(f, p.y, o.y);
+                o.z = __builtin_fmaf(f, p.z, o.z);
+                o.w = __builtin_fmaf(f, p.w, o.w);
+            }
+        }
+        if constexpr (G > 1) {
+            *reinterpret_cast<float4 *>(&part[g][r][d]) = o;
+            __syncthreads();
+            if (g == 0) {
+#pragma unroll
+                for (int k = 1; k < G; ++k) {
+                    const float4 p = *reinterpret_cast<const float4 *>(&part[k][r][d]);
+                    o.x += p.x;
+                    o.y += p.y;
+                    o.z += p.z;
+                    o.w += p.w;
+                }
+            }
+        }
+        if (live && g == 0) {
+            const float L = total[r], inv = 1.0f / L;
+            *reinterpret_cast<float4 *>(a.out + (row0 + i0 + r) * HD + d) =
+                L > 0 ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0, 0, 0, 0);
+        }
+        __syncthreads();
+    }
 }
 
-// Block (256 slots, kv head, unit); the last block of x joins the kv head's rows instead.
-__global__ __launch_bounds__(256) void span_record_kernel(SpanRecordArgs r, int HD) {
+template <int HD, int G>
+__global__ __launch_bounds__(256) void span_join_kernel(SpanArgs a, int64_t rows) {
+    constexpr int kRows = 256 / (G * (HD / 4));
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
+    join_rows<HD, G>(a, row0, static_cast<int>(min(static_cast<int64_t>(kRows), rows - row0)));
+}
+
+// Block (256 slots, kv head, unit); the first block of x joins the kv head's rows instead.
+template <int HD, int G>
+__global__ __launch_bounds__(256) void span_record_kernel(SpanRecordArgs r) {
     const SpanArgs &a = r.a;
     const int kh = blockIdx.y, unit = blockIdx.z, t = threadIdx.x;
     const size_t row0 = static_cast<size_t>(unit) * a.heads + kh * a.group;
-    if (blockIdx.x == gridDim.x - 1) {
-        const int per = HD / 4;
-        for (int i = t; i < a.group * per; i += 256) join_row(a, HD, row0 + i / per, i % per * 4);
+    if (blockIdx.x == 0) {
+        join_rows<HD, G>(a, row0, a.group);
         return;
     }
     __shared__ float2 all[kSpanMaxGroup];
-    if (t < a.group) all[t] = join_ml(a.rec_ml + (row0 + t) * a.splits_total, a.splits_total);
-    __syncthreads();
     const int n = min(a.lengths ? a.lengths[unit] : a.length, a.length);
-    const int slot = blockIdx.x * 256 + t;
+    if (static_cast<int>(blockIdx.x - 1) * 256 >= n) return;
+    for (int g = t >> 6; g < a.group; g += 4) {
+        const float2 v = join_sums(a, row0 + g, t & 63, nullptr);
+        if ((t & 63) == 0) all[g] = v;
+    }
+    __syncthreads();
+    const int slot = (blockIdx.x - 1) * 256 + t;
     if (slot >= n) return;
     const float *x = a.scores + row0 * a.score_stride + slot;
     float sum = 0.0f;
@@ -525,16 +512,44 @@ void launch_span(const SpanArgs &a, int head_dim, hipStream_t s) {
     }
 }
 
+namespace {
+
+// F(head_dim, groups that share a row's records)
+template <class F>
+void with_join(int head_dim, int splits, F &&f) {
+    auto groups = [&](auto hd) {
+        if (splits <= 1) f(hd, std::integral_constant<int, 1>{});
+        else if (splits <= 2) f(hd, std::integral_constant<int, 2>{});
+        else if (splits <= 4) f(hd, std::integral_constant<int, 4>{});
+        else f(hd, std::integral_constant<int, 8>{});
+    };
+    switch (head_dim) {
+    case 32: groups(std::integral_constant<int, 32>{}); break;
+    case 64: groups(std::integral_constant<int, 64>{}); break;
+    default: groups(std::integral_constant<int, 128>{}); break;
+    }
+}
+
+}  // namespace
+
 void launch_span_join(const SpanArgs &a, int head_dim, hipStream_t s) {
+    ND_CHECK(a.splits_total <= kJoinMax, "attention: too many pieces");
     const int64_t rows = static_cast<int64_t>(a.units) * a.count * a.heads;
-    const int per = 256 / (head_dim / 4);
-    hipLaunchKernelGGL(span_join_kernel, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(256), 0, s, a, head_dim, rows);
+    with_join(head_dim, a.splits_total, [&](auto hd, auto groups) {
+        constexpr int HD = decltype(hd)::value, G = decltype(groups)::value;
+        constexpr int kRows = 256 / (G * (HD / 4));
+        hipLaunchKernelGGL((span_join_kernel<HD, G>), dim3(static_cast<unsigned>((rows + kRows - 1) / kRows)), dim3(256), 0, s,
+                           a, rows);
+    });
     ND_HIP(hipGetLastError());
 }
 
 void launch_span_record(const SpanRecordArgs &r, int head_dim, hipStream_t s) {
+    ND_CHECK(r.a.splits_total <= kJoinMax, "attention: too many pieces");
     const dim3 grid((r.a.length + 255) / 256 + 1, r.a.kvheads, r.a.units);
-    hipLaunchKernelGGL(span_record_kernel, grid, dim3(256), 0, s, r, head_dim);
+    with_join(head_dim, r.a.splits_total, [&](auto hd, auto groups) {
+        hipLaunchKernelGGL((span_record_kernel<decltype(hd)::value, decltype(groups)::value>), grid, dim3(256), 0, s, r);
+    });
     ND_HIP(hipGetLastError());
 }
 

@@ -1,5 +1,12 @@
 // gfx950 kernel of span attention with many query rows over the same keys: prompt pieces, and a batch over its shared
-// prefix. The mathematics and the records are span_kernels.hip's; both products run on v_mfma_f32_32x32x16_bf16.
+// prefix. The mathematics and the records are span_kernels.hip's. The matrix instructions bound this kernel, so both
+// products run on v_mfma_f32_32x32x16_f16 with q and p * vs as two float16 terms (the codes are float16 numbers as they
+// are) instead of three bfloat16 ones: 22 bits of a value, and of small values what lies above 2^-25 of the term's unit.
+//   q is scaled by a power of two so that the row's largest |q| is in [2^14, 2^15). What the terms leave is below 2^-25
+//   there, 2^-25 * 127 HD * |ks| in a score; where that could pass 2^-24 (of a score times log2 e, whose own rounding is
+//   2^-24 of its size) the tile's scores get the rest of q in further terms, until nothing is left.
+//   p * vs is scaled so that the largest of a row's 32 in a tile is at least 2^2: what the terms leave is below 2^-27 of
+//   it, where an fp32 sum of the 32 rounds by 2^-24 of its largest term.
 #include "span_dev.h"
 
 namespace nd {
@@ -7,20 +14,97 @@ namespace nd {
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ f32x16 mfma32(const u32x4 &a, const u32x4 &b, const f32x16 &c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// A wave's running maximum moves only when a score is this much above it (powers of two): weights up to 2^kSlack are as
-// exact as weights up to 1, and most tiles leave the outputs unscaled.
-constexpr float kSlack = 16.0f;
+// x - h of the lower or upper float16 of a pair (exact where h is x rounded).
+__device__ __forceinline__ float less_low(uint32_t h, float x) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
+__device__ __forceinline__ float less_high(uint32_t h, float x) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t round_pair(float a, float b) {
+    const f16x2 h = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+    return __builtin_bit_cast(uint32_t, h);
+}
+
+// Two float16 terms of eight values.
+struct Halves {
+    u32x4 hi, lo;
+};
+__device__ __forceinline__ Halves halve8(const float (&x)[8]) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h[i] = round_pair(x[2 * i], x[2 * i + 1]);
+        l[i] = round_pair(less_low(h[i], x[2 * i]), less_high(h[i], x[2 * i + 1]));
+    }
+    return Halves{u32x4{h[0], h[1], h[2], h[3]}, u32x4{l[0], l[1], l[2], l[3]}};
+}
+// and what they leave, exactly
+__device__ __forceinline__ Halves take8(float (&x)[8]) {
+    const Halves t = halve8(x);
+    const uint32_t h[4] = {t.hi.x, t.hi.y, t.hi.z, t.hi.w}, l[4] = {t.lo.x, t.lo.y, t.lo.z, t.lo.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = less_low(l[i], less_low(h[i], x[2 * i]));
+        x[2 * i + 1] = less_high(l[i], less_high(h[i], x[2 * i + 1]));
+    }
+    return t;
+}
+// The same where values may be infinite or NaN: those are their first term alone.
+__device__ __forceinline__ Halves halve8_any(const float (&x)[8]) {
+    float y[8], z[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const bool odd = !(fabsf(x[i]) < INFINITY);
+        y[i] = odd ? 0.0f : x[i];
+        z[i] = odd ? x[i] : y[i];
+    }
+    return Halves{halve8(z).hi, halve8(y).lo};
+}
+
+// Two codes as float16 (exact).
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+// Eight codes of two dwords as float16: a byte b = code + 128 under the exponent of 1024 is 1024 + b.
+__device__ __forceinline__ u32x4 widen_half(uint32_t a, uint32_t b) {
+    const uint32_t w[2] = {a ^ 0x80808080u, b ^ 0x80808080u};
+    const f16x2 off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t p = __builtin_amdgcn_perm(w[i / 2], 0x64646464u, i % 2 ? 0x00070006u : 0x00050004u);
+        r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, p) + off);
+    }
+    return u32x4{r[0], r[1], r[2], r[3]};
+}
+
+// The row's outputs and sum are held times 2^(kLift - M): M is a whole number, at least the largest score (times log2 e)
+// plus the exponent of its tile's largest V scale, less kSlack (so it moves, and the outputs are rescaled, in few tiles).
+// For a tile that lies kDrop or more below M for some row the outputs are scaled up to that tile's own largest weights and
+// back, by powers of two: exactly.
+constexpr float kLift = 10.0f, kSlack = 5.0f, kDrop = 8.0f;
+constexpr int kMostExp = 50;  // of a V scale that M follows: the sum, which M scales too, stays far from underflow
+constexpr int kMostUp = 80;   // of a scaling to a tile's own weights: the outputs stay far from overflow
 
 constexpr int kFrag = 66;  // 16-byte lanes of an operand in LDS: 32, one of padding (the halves in different banks), 32, 1
 __device__ __forceinline__ int frag_lane(int m, int half) { return m + 33 * half; }
 
 // Block (W row groups of 32 and piece, with unit and kv head): W waves over the same tiles of 32 keys, which the block
-// turns into bfloat16 operands in LDS once, the next tile's codes in flight meanwhile (two buffers, one barrier a tile).
+// turns into float16 operands in LDS once. A wave forms the next tile's scores while it does this tile's softmax and
+// values, so that the matrix unit and the vector unit of a SIMD work at once: K is in LDS two tiles ahead of its values,
+// codes are a tile further ahead in registers, and there is one barrier a tile.
 //   Scores: operand A is 32 keys' codes, operand B the wave's 32 rows of q. Lane l holds row l % 32 and of each 32 keys
 //   8 (i / 4) + 4 (l / 32) + i % 4, i < 16.
 //   Values: operand B is p * vs straight from those registers, operand A the V codes in the same order of keys. Result t
@@ -34,7 +118,8 @@ __global__ __launch_bounds__(64 * W, 2) void span_wide_kernel(SpanArgs a) {
     constexpr int C = (kChunks + T - 1) / T;        // of each per thread
     __shared__ u32x4 kf[2][KS][kFrag];
     __shared__ u32x4 vf[2][2][DT][kFrag];
-    __shared__ __attribute__((aligned(16))) float sc[2][2][kWideTile];  // K (times scale) and V scales
+    __shared__ __attribute__((aligned(16))) float sc[4][2][kWideTile];  // K (times scale) and V scales, by tile modulo 4
+    __shared__ int sve[4];                          // exponent of the largest finite V scale of the tile's attended slots
 
     const int t = threadIdx.x, lane = t & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -72,36 +157,55 @@ __global__ __launch_bounds__(64 * W, 2) void span_wide_kernel(SpanArgs a) {
     const auto rks = buffer_rsrc(a.c.ks + row0, static_cast<uint32_t>(cap) * 4u);
     const auto rvs = buffer_rsrc(a.c.vs + row0, static_cast<uint32_t>(cap) * 4u);
 
-    // A tile's codes on their way to LDS: K as 16 dimensions of a key, V as 8 dimensions of 4 keys. Loads past the
-    // cache's rows read zero.
-    struct Raw {
+    // Codes on their way to LDS: K as 16 dimensions of a key, V as 4 dimensions of 4 keys. Loads past the cache's rows
+    // read zero.
+    struct RawK {
         u32x4 k[C];
-        uint32_t v[C][4];
         float s[2];  // K and V scale of key `col`
     };
-    auto fetch = [&](Raw &r, int tile) {
+    struct RawV {
+        uint32_t v[C][4];
+    };
+    auto fetch_k = [&](RawK &r, int tile) {
         const uint32_t s0 = static_cast<uint32_t>(slot0(tile));
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int c = t + i * T, keys = c / (HD / 4), dims = c % (HD / 4);
-            r.k[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, s0 * HD + c * 16, 0, 0);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                r.v[i][j] = __builtin_amdgcn_raw_buffer_load_b32(rv, (s0 + 4 * keys + j) * HD + dims * 4, 0, 0);
-        }
+        for (int i = 0; i < C; ++i) r.k[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, s0 * HD + (t + i * T) * 16, 0, 0);
         const uint32_t at = (s0 + col) * 4u;
         r.s[0] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rks, at, 0, 0));
         r.s[1] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rvs, at, 0, 0));
     };
-    auto place = [&](const Raw &r, int buf) {
+    auto fetch_v = [&](RawV &r, int tile) {
+        const uint32_t s0 = static_cast<uint32_t>(slot0(tile));
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            const int c = t + i * T;
+            const int c = t + i * T, keys = c / (HD / 4), dims = c % (HD / 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                r.v[i][j] = __builtin_amdgcn_raw_buffer_load_b32(rv, (s0 + 4 * keys + j) * HD + dims * 4, 0, 0);
+        }
+    };
+    auto place_k = [&](const RawK &r, int tile) {
+        const int buf = (tile - begin) & 1, sb = (tile - begin) & 3;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int c = t + i * T, key = c / KS, step = c % KS;
             if (kChunks % T != 0 && c >= kChunks) break;
-            const int key = c / KS, step = c % KS;
-            kf[buf][step][frag_lane(key, 0)] = widen(r.k[i].x, r.k[i].y);
-            kf[buf][step][frag_lane(key, 1)] = widen(r.k[i].z, r.k[i].w);
-            const int keys = c / (HD / 4), dims = c % (HD / 4);  // 4 keys: half and quarter of a step's depth
+            kf[buf][step][frag_lane(key, 0)] = widen_half(r.k[i].x, r.k[i].y);
+            kf[buf][step][frag_lane(key, 1)] = widen_half(r.k[i].z, r.k[i].w);
+        }
+        if (wave == 0) {
+            sc[sb][half][col] = half ? r.s[1] : r.s[0] * a.scale;
+            const float v = fabsf(r.s[1]);
+            const float most = group_max<32>(v < INFINITY && slot0(tile) + col < stop(tile) ? v : 0.0f, lane);
+            if (lane == 0) sve[sb] = most > 0 ? __builtin_amdgcn_frexp_expf(most) : 0;
+        }
+    };
+    auto place_v = [&](const RawV &r, int tile) {
+        const int buf = (tile - begin) & 1;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int c = t + i * T, keys = c / (HD / 4), dims = c % (HD / 4);  // 4 keys: half and quarter of a step's depth
+            if (kChunks % T != 0 && c >= kChunks) break;
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 float f[4];
@@ -109,59 +213,131 @@ __global__ __launch_bounds__(64 * W, 2) void span_wide_kernel(SpanArgs a) {
                 for (int j = 0; j < 4; ++j) f[j] = code(r.v[i][j], b);
                 const int d = dims * 4 + b;
                 u32x2 *to = reinterpret_cast<u32x2 *>(&vf[buf][keys / 4][d % DT][frag_lane(d / DT, keys & 1)]);
-                to[(keys >> 1) & 1] = u32x2{upper_halves(f[0], f[1]), upper_halves(f[2], f[3])};
+                to[(keys >> 1) & 1] = u32x2{half_pair(f[0], f[1]), half_pair(f[2], f[3])};
             }
         }
-        if (wave == 0) sc[buf][half][col] = half ? r.s[1] : r.s[0] * a.scale;
     };
 
-    Raw raw;
-    fetch(raw, begin);
+    RawK rk_next, rk_first;
+    RawV rv_next;
+    fetch_k(rk_first, begin);
+    fetch_k(rk_next, begin + 1);
+    fetch_v(rv_next, begin);
 
     // q as operand B: lane (row col, half) holds dimensions 16 c + 8 half .. of step c
     const size_t orow = (static_cast<size_t>(unit) * a.count + (live ? row : 0) / a.group) * a.heads + kh * a.group +
                         (live ? row : 0) % a.group;
-    Terms q[KS];
+    const float4 *src = reinterpret_cast<const float4 *>(a.q + orow * HD + half * 8);
+    Halves q[KS];
+    int lift;     // q is held times 2^lift
+    float down;   // 2^-lift; NaN for a row with an infinity or NaN, whose scores it makes NaN
+    float worst;  // a tile whose |K scale| (times a.scale) is above 1 / worst takes further terms of q
     {
-        const float4 *src = reinterpret_cast<const float4 *>(a.q + orow * HD + half * 8);
+        float x[KS][8];
+        float most = 0.0f;
+        bool finite = true;
 #pragma unroll
         for (int c = 0; c < KS; ++c) {
             const float4 u = src[4 * c], w = src[4 * c + 1];
             const float both[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-            float x[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = live ? both[j] : 0.0f;
-            q[c] = split8(x);
+            for (int j = 0; j < 8; ++j) {
+                x[c][j] = live ? both[j] : 0.0f;
+                finite = finite && fabsf(x[c][j]) < INFINITY;
+                most = fmaxf(most, fabsf(x[c][j]));
+            }
+        }
+        most = fmaxf(most, butterfly_partner<32>(most, lane));
+        finite = butterfly_partner<32>(finite ? 1.0f : 0.0f, lane) != 0.0f && finite;
+        lift = finite && most > 0 ? min(15 - __builtin_amdgcn_frexp_expf(most), 120) : 0;
+        down = finite ? ldexpf(1.0f, -lift) : __builtin_nanf("");
+        worst = wave_max(finite && most > 0 ? down : 0.0f, lane) * (127.0f * HD * 0.5f);
+#pragma unroll
+        for (int c = 0; c < KS; ++c) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[c][j] = finite ? ldexpf(x[c][j], lift) : 0.0f;
+            q[c] = halve8(x[c]);
         }
     }
 
-    float m = -INFINITY, l = 0.0f;
+    float M = -INFINITY, l = 0.0f;
     f32x16 acc[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
 
-    auto compute = [&](int buf, int tile) {
-        const int s0 = slot0(tile), behind = stop(tile);
+    // q times a tile's K codes, both terms (times 2^lift)
+    auto product = [&](int tile) {
+        const int buf = (tile - begin) & 1;
         f32x16 x;
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = 0.0f;
 #pragma unroll
         for (int c = 0; c < KS; ++c) {
             const u32x4 k = kf[buf][c][frag_lane(col, half)];
-            x = mfma32(k, q[c].t[2], x);
-            x = mfma32(k, q[c].t[1], x);
-            x = mfma32(k, q[c].t[0], x);
+            x = mfma32(k, q[c].lo, x);
+            x = mfma32(k, q[c].hi, x);
         }
-        const bool odd = __any(!(fabsf(sc[buf][1][col]) < INFINITY));  // an infinite or NaN V scale
+        return x;
+    };
+    // and the rest of q where it could matter
+    auto finish_product = [&](f32x16 &x, int tile) {
+        if (!__any(fabsf(sc[(tile - begin) & 3][0][col]) * worst > 1.0f)) return;
+        bool left = true;
+#pragma unroll 1
+        for (int round = 1; __any(left); ++round) {
+            left = false;
+            f32x16 e;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) e[j] = 0.0f;
+#pragma unroll 1
+            for (int c = 0; c < KS; ++c) {
+                const float4 u = src[4 * c], w = src[4 * c + 1];
+                float r[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[j] = live && down == down ? ldexpf(r[j], lift) : 0.0f;
+#pragma unroll 1
+                for (int i = 0; i < round; ++i) {  // what the terms before leave
+                    take8(r);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) r[j] *= 0x1p24f;
+                }
+                const Halves h = take8(r);
+                const u32x4 k = kf[(tile - begin) & 1][c][frag_lane(col, half)];
+                e = mfma32(k, h.lo, e);
+                e = mfma32(k, h.hi, e);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) left = left || r[j] != 0.0f;
+            }
+            const float unit = ldexpf(1.0f, -24 * round);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = __builtin_fmaf(e[j], unit, x[j]);
+        }
+    };
+
+    place_k(rk_first, begin);
+    place_k(rk_next, begin + 1);
+    place_v(rv_next, begin);
+    fetch_k(rk_next, begin + 2);
+    fetch_v(rv_next, begin + 1);
+    __syncthreads();
+    f32x16 next = product(begin);
+    finish_product(next, begin);
+    __syncthreads();  // every wave has its first scores before K's buffer is written again
+    for (int tile = begin; tile < end; ++tile) {
+        const int vb = (tile - begin) & 1, sb = (tile - begin) & 3;
+        const int s0 = slot0(tile), behind = stop(tile);
+        const bool odd = __any(!(fabsf(sc[sb][1][col]) < INFINITY));  // an infinite or NaN V scale
+        const int ve = __builtin_amdgcn_readfirstlane(sve[sb]);
+        f32x16 x;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const float4 ks = *reinterpret_cast<const float4 *>(&sc[buf][0][8 * g + 4 * half]);
-            x[4 * g] *= ks.x;
-            x[4 * g + 1] *= ks.y;
-            x[4 * g + 2] *= ks.z;
-            x[4 * g + 3] *= ks.w;
+            const float4 ks = *reinterpret_cast<const float4 *>(&sc[sb][0][8 * g + 4 * half]);
+            x[4 * g] = next[4 * g] * ks.x;
+            x[4 * g + 1] = next[4 * g + 1] * ks.y;
+            x[4 * g + 2] = next[4 * g + 2] * ks.z;
+            x[4 * g + 3] = next[4 * g + 3] * ks.w;
         }
         bool masked = s0 + kWideTile > behind;
         if constexpr (RING) {
@@ -188,56 +364,79 @@ __global__ __launch_bounds__(64 * W, 2) void span_wide_kernel(SpanArgs a) {
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 16; ++j) top = fmaxf(top, x[j]);
-        top = fmaxf(top, butterfly_partner<32>(top, lane));
-        if (__any(top > m + kSlack)) {  // (m = -inf: the first scores)
-            const float mn = fmaxf(m, top);
-            const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
+        top = fmaxf(top, butterfly_partner<32>(top, lane)) * down;
+        const int follow = max(-kMostExp, min(kMostExp, ve));
+        const float high = ceilf(top) + static_cast<float>(follow);
+        if (__any(high > M + kSlack)) {  // (M = -inf: the first scores)
+            const float most = fmaxf(M, high);
+            const float alpha = M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - most);
+            M = most;
             l *= alpha;
 #pragma unroll
             for (int i = 0; i < DT; ++i) acc[i] *= alpha;
         }
-        const float base = m == -INFINITY ? 0.0f : m;
+        const int beyond = ve - follow;
+        const bool apart = beyond != 0 || __any(high < M - kDrop && high > -INFINITY);
+        float up = 0.0f;
+        if (apart) {
+            up = high > -INFINITY ? fminf(M - high, static_cast<float>(min(kMostUp, kMostUp + beyond))) : 0.0f;
+            l *= __builtin_amdgcn_exp2f(up);
+            const float grow = __builtin_amdgcn_exp2f(up - static_cast<float>(beyond));
+#pragma unroll
+            for (int i = 0; i < DT; ++i) acc[i] *= grow;
+        }
+        const float lifted = M > -INFINITY ? kLift + up - M : 0.0f;  // nothing attended yet: every power is 0
+        // the next tile's product beside this tile's weights
+        next = product(tile + 1);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const float4 v4 = *reinterpret_cast<const float4 *>(&sc[buf][1][8 * g + 4 * half]);
+            const float4 v4 = *reinterpret_cast<const float4 *>(&sc[sb][1][8 * g + 4 * half]);
             const float vs[4] = {v4.x, v4.y, v4.z, v4.w};
+            float p[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const float p = __builtin_amdgcn_exp2f(x[4 * g + u] - base);
-                l += p;
-                x[4 * g + u] = p * vs[u];
+                p[u] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[4 * g + u], down, lifted));
+                x[4 * g + u] = p[u] * vs[u];
             }
+            l += (p[0] + p[1]) + (p[2] + p[3]);
         }
-        if (masked) {  // whatever scale a masked slot has
-#pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = gone >> j & 1u ? 0.0f : x[j];
-        }
+        Halves p[2];
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             float w[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) w[j] = x[8 * ks + j];
-            const Terms p = odd ? split8_any(w) : split8(w);
+            p[ks] = halve8(w);
+        }
+        if (odd || beyond != 0) {  // scales that are no numbers or far from 1: masked weights may be NaN, others infinite
+            const float shrink = __builtin_amdgcn_exp2f(static_cast<float>(-beyond));
 #pragma unroll
-            for (int i = 0; i < DT; ++i) {
-                const u32x4 v = vf[buf][ks][i][frag_lane(col, half)];
-                acc[i] = mfma32(v, p.t[2], acc[i]);
-                acc[i] = mfma32(v, p.t[1], acc[i]);
-                acc[i] = mfma32(v, p.t[0], acc[i]);
+            for (int ks = 0; ks < 2; ++ks) {
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = gone >> (8 * ks + j) & 1u ? 0.0f : x[8 * ks + j] * shrink;
+                p[ks] = halve8_any(w);
             }
         }
-    };
-
-    int buf = 0;
-    place(raw, buf);
-    __syncthreads();
-    for (int tile = begin; tile < end; ++tile) {
-        fetch(raw, tile + 1);
-        asm volatile("" ::: "memory");
-        compute(buf, tile);
-        buf ^= 1;
-        place(raw, buf);
+        // this tile's values beside the operands of the tiles to come
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+            for (int i = 0; i < DT; ++i) acc[i] = mfma32(vf[vb][ks][i][frag_lane(col, half)], p[ks].lo, acc[i]);
+#pragma unroll
+            for (int i = 0; i < DT; ++i) acc[i] = mfma32(vf[vb][ks][i][frag_lane(col, half)], p[ks].hi, acc[i]);
+        }
+        place_v(rv_next, tile + 1);
+        place_k(rk_next, tile + 2);
+        if (apart) {
+            l *= __builtin_amdgcn_exp2f(-up);
+            const float back = __builtin_amdgcn_exp2f(static_cast<float>(beyond) - up);
+#pragma unroll
+            for (int i = 0; i < DT; ++i) acc[i] *= back;
+        }
+        finish_product(next, tile + 1);
+        fetch_k(rk_next, tile + 3);
+        fetch_v(rv_next, tile + 2);
         __syncthreads();
     }
 
@@ -248,7 +447,7 @@ __global__ __launch_bounds__(64 * W, 2) void span_wide_kernel(SpanArgs a) {
     float *to = finish ? a.out + orow * HD : a.rec_o + rec * HD;
     const float inv = !finish ? 1.0f : l > 0 ? 1.0f / l : 0.0f;
     const bool none = finish && !(l > 0);  // nothing attended, or no softmax
-    if (!finish && half == 0) a.rec_ml[rec] = make_float2(m, l);
+    if (!finish && half == 0) a.rec_ml[rec] = make_float2(M - kLift, l);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
         const int d = DT * (8 * (j / 4) + 4 * half + j % 4);

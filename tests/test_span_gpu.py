@@ -235,6 +235,80 @@ def test_non_finite_input():
             np.testing.assert_array_equal(got[0, 0, h], want)
 
 
+# ---- many rows over the same keys: two float16 terms ----------------------------------------------------------------
+def check_many_rows(r, q, first, got):
+    """A prompt piece over a window of first + 1 positions, the first token's from position 0 on (slot = position, tiles of
+    32 slots): the tolerance above, whose sums have room for the terms' 2^-22 per value and 2^-24 per score, plus what the terms of a weight leave: at most
+    2^-27 of the largest p * v_scale among the tile's 32."""
+    kvh, hd = r.k.shape[2], q.shape[-1]
+    group = q.shape[2] // kvh
+    for i in range(q.shape[1]):
+        at = np.arange(i, first + i + 1)
+        for h in range(kvh):
+            k, v = r.at(0, at, h)
+            vs, codes = np.abs(r.vs[0, at, h].astype(np.float64)), np.abs(r.v[0, at, h].astype(np.float64))
+            for g in range(group):
+                want, tol, p = attend(q[0, i, h * group + g], k, v)
+                for t in np.unique(at // 32):
+                    mine = at // 32 == t
+                    tol = tol + 2.0 ** -27 * (p[mine] * vs[mine]).max() * codes[mine].sum(0)
+                check(got[0, i, h * group + g], want, tol, f"token {i} head {h * group + g}")
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("ratio", [1e4, 1e6, 1e8, 1e12, 1e30])
+def test_many_rows_uneven_queries(hd, ratio):
+    """Entries of q far above the rest over zero K codes, in some rows only: the other entries' products decide."""
+    rng = np.random.default_rng(hd + int(np.log10(ratio)))
+    r = Rows(rng, 1, 340, 2, hd)
+    r.k[:, :, :, 5] = 0
+    r.push()
+    q = rng.normal(size=(1, 40, 4, hd)).astype(np.float32)
+    q[0, 3::7, :, 5] = ratio
+    q[0, 5] *= 1e-30
+    q[0, 6] = 0
+    check_many_rows(r, q, 300, run_window(r, q, [300], 0, 301))
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("margin", [3, 10, 30, 60, 120])
+def test_many_rows_dominant_slots(hd, margin):
+    """Some slots whose scores are `margin` above the rest, with zero V codes in half of the dimensions: there the other
+    slots' sums show, down to e^-120 of the weights (the smallest normal number is e^-87: less is lost, within 1e-37)."""
+    rng = np.random.default_rng(hd + margin)
+    r = Rows(rng, 1, 340, 2, hd)
+    sign = rng.choice([-1, 1], hd)
+    q = (np.abs(rng.normal(size=(1, 40, 4, hd))) * sign).astype(np.float32)
+    for j in (0, 77, 200):
+        r.k[0, j] = 127 * sign
+        r.ks[0, j] = margin * np.sqrt(hd) / (127 * np.abs(q).sum(-1).mean())
+        r.v[0, j, :, ::2] = 0
+    r.push()
+    check_many_rows(r, q, 300, run_window(r, q, [300], 0, 301))
+
+
+@pytest.mark.parametrize("scales", ["tiny", "huge", "mixed", "zero", "signed"])
+def test_many_rows_v_scales(scales):
+    rng = np.random.default_rng(50)
+    r = Rows(rng, 1, 340, 2, 64)
+    if scales == "tiny":
+        r.vs *= np.float32(2.0 ** -108)
+    elif scales == "huge":
+        r.vs *= np.float32(2.0 ** 118)
+    elif scales == "mixed":
+        r.vs[0, :160] *= np.float32(2.0 ** -100)
+        r.vs[0, 100] = 2.0 ** 90
+        r.vs[0, 200:] *= np.float32(2.0 ** -30)
+    elif scales == "zero":
+        r.vs[0, :200] = 0
+    else:
+        r.vs[0, ::3] *= -1
+        r.ks[0, ::2] *= -1
+    r.push()
+    q = rng.normal(size=(1, 40, 4, 64)).astype(np.float32)
+    check_many_rows(r, q, 300, run_window(r, q, [300], 0, 301))
+
+
 # ---- a shared prefix ----------------------------------------------------------------------------------------------
 def run_shared(r, prefix, prefix_length, q, length, lengths, new=None, prefix_seq=0, stream=None):
     out = DeviceArray.from_host(np.full(q.shape, np.nan, np.float32))

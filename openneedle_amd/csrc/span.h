@@ -30,12 +30,15 @@ struct SpanArgs {
     // A unit's tiles (span_geom.h) are cut into `splits` pieces of `per` tiles; piece s leaves record split0 + s of a row's
     // splits_total. Without records (one piece) the rows are finished in place.
     int splits, per, split0, splits_total;
+    int waves;             // of a block of 16 rows: 4 or 8
+    int groups;            // row groups of 32 of a block of the wide kernel, 1 to 4
     float *rec_o;          // nullable, [rows][splits_total][head_dim]
     float2 *rec_ml;        // [rows][splits_total]: running maximum (of scores times log2 e) and sum
     float *scores;         // nullable: [unit][kvh][group][score_stride] scores times log2 e (count 1, no ring)
     int score_stride;      // a whole number of tiles
     float scale;           // log2(e) / sqrt(head_dim)
-    // count 1: one new token per unit (null: none), [units][kvheads][head_dim], stored in the unit's last attended slot
+    // launch_span, at most 16 rows a unit: the tokens' own rows (null: stored already), [units][count][kvheads][head_dim],
+    // stored at their ring slots, or (no ring, count 1) in the unit's last attended slot, before they are attended
     const float *new_k, *new_v;
 };
 
@@ -57,9 +60,12 @@ struct SpanRecordArgs {
 constexpr int kSpanRows = 16;      // query rows of a block
 
 void launch_span_store(const SpanStoreArgs &a, hipStream_t s);
+// Blocks of 16 query rows; and of 32 * groups, whose keys are turned into operands once for them all.
 void launch_span(const SpanArgs &a, int head_dim, hipStream_t s);
-// the same in blocks of 32 * waves query rows (waves 1 to 4)
-void launch_span_wide(const SpanArgs &a, int head_dim, int waves, hipStream_t s);
+void launch_span_wide(const SpanArgs &a, int head_dim, hipStream_t s);
+// A shared prefix (one unit, no ring), as either of them, and the units' own keys (at most 16 rows each) in one launch.
+void launch_span_two(const SpanArgs &far, const SpanArgs &own, int head_dim, hipStream_t s);
+void launch_span_wide_own(const SpanArgs &far, const SpanArgs &own, int head_dim, hipStream_t s);
 // out rows from all their records
 void launch_span_join(const SpanArgs &a, int head_dim, hipStream_t s);
 void launch_span_record(const SpanRecordArgs &a, int head_dim, hipStream_t s);

@@ -41,40 +41,73 @@ static SpanArgs span_args(KvHandle &kv, const SpanCache &c, const float *d_q, fl
     return a;
 }
 
-// How a launch is cut: `waves` 0 for the 16-row kernel, else the wide kernel's row groups of 32 per block.
-struct SpanPlan {
-    int waves = 0;
+// How a launch is cut, by estimates (us) from measurements at 256 compute units. A round of a 16-row block (a tile of 64
+// keys per wave) takes 1.2 / 1.25 / 1.85 for rows of 32 / 64 / 128 values with at most one block per unit, of four or
+// eight waves, and 1.6 / 2.4 / 4.1 with two of four; a tile of a wide block (32 keys) 1.15 / 1.15 / 1.2 and
+// 1.5 / 1.7 / 2.3. Blocks start and end in 5 (eight waves 5.8, wide 6), a join launch takes 3.5, records are written and
+// read at 3 TB/s, a piece of a 16-row block costs 0.5 more, and a unit takes its keys at 20 GB/s.
+struct Rate {
+    int waves;               // of a block
+    int tiles;               // of a round
+    double start, one, two;  // us a block, and a round with one block per compute unit and with two (0: never two)
+};
+struct Cut {
+    double us = 0;
+    int splits = 1, per = 1, waves = 4;
 };
 
-// Pieces of a unit's keys (at most `keys` in `runs` runs): two blocks per compute unit, of whole rounds of a block.
-static SpanPlan cut(SpanArgs &a, int keys, int runs) {
-    const int64_t rows = int64_t(a.count) * a.group;
-    SpanPlan p;
-    if (rows > kSpanRows) {
-        double best = 0;
-        for (int w = 4; w >= 1; --w) {
-            const double cost = double((rows + 32 * w - 1) / (32 * w)) * (w + 0.6);
-            if (!p.waves || cost < best) {
-                best = cost;
-                p.waves = w;
-            }
-        }
+// The cheapest cut of blocks of `tiles` tiles and `bytes` each, `blocks` of them without pieces.
+static void best_cut(Cut &best, int64_t blocks, int tiles, double bytes, const Rate &r, double record, double join) {
+    const int cus = device_cus(), room = r.two > 0 ? 2 * cus : cus;
+    const int rounds = (tiles + r.tiles - 1) / r.tiles;
+    const int most = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rounds, room / blocks)));
+    for (int s = 1;; s = std::min(most, s < 4 ? s + 1 : s + s / 3)) {
+        const int64_t n = s * blocks;
+        const int per = (rounds + s - 1) / s;
+        const bool one = n <= cus;
+        if (!one && r.two == 0) return;
+        const double flights = one ? 1 : double((n + room - 1) / room);
+        const double stream = blocks * bytes / (double(std::min<int64_t>(n, cus)) * 2e4);
+        const double us = std::max(stream, flights * (r.start + per * (one ? r.one : r.two))) + (s > 1 ? join : 0) + s * record;
+        if (best.us == 0 || us < best.us) best = Cut{us, (rounds + per - 1) / per, per * r.tiles, r.waves};
+        if (s >= most) return;
     }
-    const int block_rows = p.waves ? 32 * p.waves : kSpanRows;
-    const int64_t blocks = std::max<int64_t>(1, (rows + block_rows - 1) / block_rows * a.kvheads * a.units);
-    const int round = p.waves ? 1 : 4;  // tiles of a block's round
-    const int tiles = (p.waves ? wide_tiles(keys) : span_tiles(keys)) + runs - 1;
-    const int rounds = std::max(1, (tiles + round - 1) / round);
-    const int target = 2 * device_cus();
-    const int want = static_cast<int>(std::min<int64_t>(rounds, std::max<int64_t>(1, target / blocks)));
-    const int per_rounds = (rounds + want - 1) / want;
-    a.per = round * per_rounds;
-    a.splits = (rounds + per_rounds - 1) / per_rounds;
-    return p;
 }
 
-static void launch(const SpanArgs &a, const SpanPlan &p, int head_dim, hipStream_t s) {
-    if (p.waves) launch_span_wide(a, head_dim, p.waves, s);
+// Cuts `a`; true: for the wide kernel. keys: at most so many per row tile of 16 (wide: of 128) rows, in `runs` runs;
+// joined: a join follows in any case.
+static bool plan(SpanArgs &a, int head_dim, int keys, int wide_keys, int runs, bool joined, bool may_wide) {
+    static const Rate kFour[3] = {{4, 4, 5, 1.2, 1.6}, {4, 4, 5, 1.25, 2.4}, {4, 4, 5, 1.85, 4.1}};
+    static const Rate kEight[3] = {{8, 8, 5.8, 1.2, 0}, {8, 8, 5.8, 1.25, 0}, {8, 8, 5.8, 1.85, 0}};
+    static const Rate kWide[3] = {{4, 1, 6, 1.15, 1.5}, {4, 1, 6, 1.15, 1.7}, {4, 1, 6, 1.2, 2.3}};
+    const int h = head_dim == 32 ? 0 : head_dim == 64 ? 1 : 2;
+    const int64_t rows = int64_t(a.count) * a.group, units = int64_t(a.units) * a.kvheads;
+    const double record = double(rows) * units * head_dim * 8 / 3e6, join = joined ? 0 : 3.5;
+    const int64_t blocks = (rows + kSpanRows - 1) / kSpanRows * units;
+    const int tiles = std::max(1, span_tiles(keys) + runs - 1);
+    const double row = 2.0 * (head_dim + 4);
+    Cut c;
+    best_cut(c, blocks, tiles, keys * row, kFour[h], record + 0.5, join);
+    best_cut(c, blocks, tiles, keys * row, kEight[h], record + 0.5, join);
+    bool wide = false;
+    if (may_wide && rows > kSpanRows) {
+        const int64_t row_blocks = (rows + 127) / 128;
+        Cut w;
+        best_cut(w, row_blocks * units, std::max(1, wide_tiles(wide_keys) + runs - 1), wide_keys * row, kWide[h], record, join);
+        wide = w.us < c.us;
+        if (wide) {
+            c = w;
+            a.groups = a.positions ? 4 : int(((rows + 31) / 32 + row_blocks - 1) / row_blocks);
+        }
+    }
+    a.splits = c.splits;
+    a.per = c.per;
+    a.waves = c.waves;
+    return wide;
+}
+
+static void launch(const SpanArgs &a, bool wide, int head_dim, hipStream_t s) {
+    if (wide) launch_span_wide(a, head_dim, s);
     else launch_span(a, head_dim, s);
 }
 
@@ -112,12 +145,14 @@ int needle2_gpu_attention_window(void *h, int layer, const float *d_q, float *d_
         a.sinks = sinks;
         a.window = window;
         // keys of a block: its tokens' windows
-        const int most = int64_t(count) * a.group <= kSpanRows ? kSpanRows : 128;
-        const int tokens = std::min(count, (most + a.group - 1) / a.group + 1);
-        const SpanPlan plan = cut(a, sinks + window + tokens - 1, 2);
+        auto keys = [&](int rows) {
+            const int64_t tokens = (rows + a.group - 1) / a.group + 1;
+            return int(std::min<int64_t>(sinks + int64_t(window) + std::min<int64_t>(count, tokens) - 1, kv.capacity));
+        };
+        const bool wide = plan(a, kv.head_dim, keys(kSpanRows), keys(128), 2, false, true);
         a.splits_total = a.splits;
         if (a.splits_total > 1) reserve_records(kv, a, int64_t(kv.seqs) * count * heads);
-        if (d_new_k && count == 1) {
+        if (d_new_k && int64_t(count) * a.group <= kSpanRows) {
             a.new_k = d_new_k;
             a.new_v = d_new_v;
         } else if (d_new_k) {
@@ -133,7 +168,7 @@ int needle2_gpu_attention_window(void *h, int layer, const float *d_q, float *d_
             st.sinks = sinks;
             launch_span_store(st, s);
         }
-        launch(a, plan, kv.head_dim, s);
+        launch(a, wide, kv.head_dim, s);
         if (a.splits_total > 1) launch_span_join(a, kv.head_dim, s);
     });
 }
@@ -158,11 +193,12 @@ int needle2_gpu_attention_shared(void *h, int layer, void *prefix, int prefix_se
         own.lengths = d_lengths;
         own.new_k = d_new_k;
         own.new_v = d_new_v;
-        const SpanPlan own_plan = cut(own, length, 1);
         SpanArgs far = span_args(kv, layer_of(pre, layer, prefix_seq), d_q, d_out, 1, heads, kv.seqs);
         far.length = prefix_length;
-        const SpanPlan far_plan = cut(far, prefix_length, 1);
-        if (prefix_length == 0) far.splits = 0;
+        const bool shared = prefix_length > 0;
+        plan(own, kv.head_dim, length, 0, 1, shared, false);
+        const bool wide = plan(far, kv.head_dim, prefix_length, prefix_length, 1, true, true);
+        if (!shared) far.splits = 0;
         own.split0 = far.splits;
         own.splits_total = far.splits_total = far.splits + own.splits;
         if (own.splits_total > 1) {
@@ -170,8 +206,16 @@ int needle2_gpu_attention_shared(void *h, int layer, void *prefix, int prefix_se
             far.rec_o = own.rec_o;
             far.rec_ml = own.rec_ml;
         }
-        if (prefix_length > 0) launch(far, far_plan, kv.head_dim, s);
-        launch(own, own_plan, kv.head_dim, s);
+        if (!shared) {
+            launch_span(own, kv.head_dim, s);
+        } else if (wide) {
+            launch_span_wide_own(far, own, kv.head_dim, s);
+        } else {
+            // eight waves fill a compute unit, and the launch has the sequences' own blocks too
+            const int64_t row_tiles = (int64_t(far.count) * far.group + kSpanRows - 1) / kSpanRows;
+            if ((row_tiles * far.splits + int64_t(own.splits) * own.units) * own.kvheads > device_cus()) far.waves = 4;
+            launch_span_two(far, own, kv.head_dim, s);
+        }
         if (own.splits_total > 1) launch_span_join(own, kv.head_dim, s);
     });
 }
@@ -191,14 +235,13 @@ int needle2_gpu_attention_weights(void *h, int layer, const float *d_q, float *d
         a.lengths = d_lengths;
         a.new_k = d_new_k;
         a.new_v = d_new_v;
-        const int tiles = span_tiles(length);
-        const SpanPlan plan = cut(a, length, 1);
+        plan(a, kv.head_dim, length, 0, 1, true, false);
         a.splits_total = a.splits;
         reserve_records(kv, a, int64_t(kv.seqs) * heads);  // for one piece too: the weights need the final sums
-        a.score_stride = std::max(1, tiles) * kSpanTile;
+        a.score_stride = std::max(1, span_tiles(length)) * kSpanTile;
         a.scores = kv.scores.reserve(size_t(kv.seqs) * heads * a.score_stride);
         SpanRecordArgs r{a, d_weights};
-        launch(a, plan, kv.head_dim, s);
+        launch_span(a, kv.head_dim, s);
         launch_span_record(r, kv.head_dim, s);
     });
 }

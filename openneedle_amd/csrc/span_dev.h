@@ -68,6 +68,38 @@ __device__ __forceinline__ u32x4 widen(uint32_t a, uint32_t b) {
                  upper_halves(code(b, 0), code(b, 1)), upper_halves(code(b, 2), code(b, 3))};
 }
 
+// A new token's K and V rows of HD values in a wave's registers, two values each a lane.
+struct NewRow {
+    float k[2], v[2];
+};
+__device__ __forceinline__ NewRow read_row(const float *k, const float *v, int HD, int lane) {
+    NewRow r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const bool in = lane + 64 * i < HD;
+        r.k[i] = in ? k[lane + 64 * i] : 0.0f;
+        r.v[i] = in ? v[lane + 64 * i] : 0.0f;
+    }
+    return r;
+}
+
+// One row into codes and scale, by one wave (the cache's quantiser: top = max|x|, scale = top / 127 or 1, codes
+// round(x * (127 / top))).
+__device__ __forceinline__ void quantise_row(const float (&x)[2], int HD, int lane, int8_t *codes, float *scale) {
+    const float top = wave_max(fmaxf(fabsf(x[0]), fabsf(x[1])), lane);
+    const float inv = top > 0 ? 127.0f / top : 0.0f;
+    if (lane == 0) *scale = top > 0 ? top / 127.0f : 1.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (lane + 64 * i < HD)
+            codes[lane + 64 * i] = static_cast<int8_t>(fmaxf(-127.0f, fminf(127.0f, rintf(x[i] * inv))));
+}
+
+__device__ __forceinline__ void store_row(const SpanCache &c, const NewRow &r, size_t row, int HD, int lane) {
+    quantise_row(r.k, HD, lane, c.k8 + row * HD, c.ks + row);
+    quantise_row(r.v, HD, lane, c.v8 + row * HD, c.vs + row);
+}
+
 __device__ __forceinline__ int at_position(int first, int i) {
     return static_cast<int>(static_cast<uint32_t>(first) + static_cast<uint32_t>(i));
 }

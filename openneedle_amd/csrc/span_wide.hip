@@ -7,7 +7,7 @@
 //   2^-24 of its size) the tile's scores get the rest of q in further terms, until nothing is left.
 //   p * vs is scaled so that the largest of a row's 32 in a tile is at least 2^2: what the terms leave is below 2^-27 of
 //   it, where an fp32 sum of the 32 rounds by 2^-24 of its largest term.
-#include "span_dev.h"
+#include "span_rows.h"
 
 namespace nd {
 
@@ -96,41 +96,46 @@ __device__ __forceinline__ u32x4 widen_half(uint32_t a, uint32_t b) {
 // back, by powers of two: exactly.
 constexpr float kLift = 10.0f, kSlack = 5.0f, kDrop = 8.0f;
 constexpr int kMostExp = 50;  // of a V scale that M follows: the sum, which M scales too, stays far from underflow
+constexpr int kOddTile = 1024;
 constexpr int kMostUp = 80;   // of a scaling to a tile's own weights: the outputs stay far from overflow
 
 constexpr int kFrag = 66;  // 16-byte lanes of an operand in LDS: 32, one of padding (the halves in different banks), 32, 1
 __device__ __forceinline__ int frag_lane(int m, int half) { return m + 33 * half; }
 
-// Block (W row groups of 32 and piece, with unit and kv head): W waves over the same tiles of 32 keys, which the block
-// turns into float16 operands in LDS once. A wave forms the next tile's scores while it does this tile's softmax and
+// Block (up to four row groups of 32 and piece, with unit and kv head): four waves over the same tiles of 32 keys, which
+// the block turns into float16 operands in LDS once; a wave without rows only helps with that (a window's blocks have
+// four groups but for the last). A wave forms the next tile's scores while it does this tile's softmax and
 // values, so that the matrix unit and the vector unit of a SIMD work at once: K is in LDS two tiles ahead of its values,
 // codes are a tile further ahead in registers, and there is one barrier a tile.
 //   Scores: operand A is 32 keys' codes, operand B the wave's 32 rows of q. Lane l holds row l % 32 and of each 32 keys
 //   8 (i / 4) + 4 (l / 32) + i % 4, i < 16.
 //   Values: operand B is p * vs straight from those registers, operand A the V codes in the same order of keys. Result t
 //   of lane l is row l % 32, dimensions DT * (8 (i / 4) + 4 (l / 32) + i % 4) + t (DT = HD / 32 results).
-template <int HD, int W, bool RING>
-__global__ __launch_bounds__(64 * W, 2) void span_wide_kernel(SpanArgs a) {
+template <int HD, bool RING>
+__device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
     constexpr int KS = HD / 16;                     // steps of the score product's depth
     constexpr int DT = HD / 32;                     // results of 32 dimensions
-    constexpr int T = 64 * W;
+    constexpr int T = 256;
     constexpr int kChunks = 2 * HD;                 // of a tile's K codes, 16 bytes each; and pieces of V, 4 keys x 4 dimensions
     constexpr int C = (kChunks + T - 1) / T;        // of each per thread
     __shared__ u32x4 kf[2][KS][kFrag];
     __shared__ u32x4 vf[2][2][DT][kFrag];
     __shared__ __attribute__((aligned(16))) float sc[4][2][kWideTile];  // K (times scale) and V scales, by tile modulo 4
-    __shared__ int sve[4];                          // exponent of the largest finite V scale of the tile's attended slots
+    // of the tile's slots in its run: the exponent of the largest finite V scale, plus kOddTile where one is infinite or
+    // NaN; and the largest |K scale|
+    __shared__ int2 about[4];
 
     const int t = threadIdx.x, lane = t & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int pairs = a.units * a.kvheads;
-    const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
+    const int pair = bx % pairs, rest = bx / pairs;
     const int unit = pair / a.kvheads, kh = pair % a.kvheads;
-    const int piece = rest % a.splits, tile_rows = rest / a.splits * (32 * W);
+    const int piece = rest % a.splits, tile_rows = rest / a.splits * (32 * a.groups);
     const int rows = a.count * a.group;
-    const int last_row = min(rows, tile_rows + 32 * W) - 1;
+    const int last_row = min(rows, tile_rows + 32 * a.groups) - 1;
+    const bool works = wave < a.groups;
     const int row = tile_rows + wave * 32 + col;
-    const bool live = row < rows;
+    const bool live = works && row < rows;
     const int cap = a.c.capacity;
 
     KeyRuns runs = {0, 0, 0, 0, 0, 0};
@@ -194,10 +199,15 @@ __global__ __launch_bounds__(64 * W, 2) void span_wide_kernel(SpanArgs a) {
             kf[buf][step][frag_lane(key, 1)] = widen_half(r.k[i].z, r.k[i].w);
         }
         if (wave == 0) {
-            sc[sb][half][col] = half ? r.s[1] : r.s[0] * a.scale;
-            const float v = fabsf(r.s[1]);
-            const float most = group_max<32>(v < INFINITY && slot0(tile) + col < stop(tile) ? v : 0.0f, lane);
-            if (lane == 0) sve[sb] = most > 0 ? __builtin_amdgcn_frexp_expf(most) : 0;
+            const bool in = slot0(tile) + col < stop(tile);
+            const float ks = in ? r.s[0] * a.scale : 0.0f, vs = in ? r.s[1] : 0.0f;
+            sc[sb][half][col] = half ? vs : ks;
+            const float v = fabsf(vs);
+            const bool odd = !(v < INFINITY);
+            const float most = group_max<32>(half ? odd ? 0.0f : v : fabsf(ks), lane);
+            const float v_most = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, most), 32));
+            const int ve = (v_most > 0 ? __builtin_amdgcn_frexp_expf(v_most) : 0) + (__any(odd) ? kOddTile : 0);
+            if (lane == 0) about[sb] = make_int2(ve, __builtin_bit_cast(int, most));
         }
     };
     auto place_v = [&](const RawV &r, int tile) {
@@ -223,6 +233,23 @@ __global__ __launch_bounds__(64 * W, 2) void span_wide_kernel(SpanArgs a) {
     fetch_k(rk_first, begin);
     fetch_k(rk_next, begin + 1);
     fetch_v(rv_next, begin);
+    if (!RING && !works) {
+        place_k(rk_first, begin);
+        place_k(rk_next, begin + 1);
+        place_v(rv_next, begin);
+        fetch_k(rk_next, begin + 2);
+        fetch_v(rv_next, begin + 1);
+        __syncthreads();
+        __syncthreads();
+        for (int tile = begin; tile < end; ++tile) {
+            place_v(rv_next, tile + 1);
+            place_k(rk_next, tile + 2);
+            fetch_k(rk_next, tile + 3);
+            fetch_v(rv_next, tile + 2);
+            __syncthreads();
+        }
+        return;
+    }
 
     // q as operand B: lane (row col, half) holds dimensions 16 c + 8 half .. of step c
     const size_t orow = (static_cast<size_t>(unit) * a.count + (live ? row : 0) / a.group) * a.heads + kh * a.group +
@@ -283,7 +310,7 @@ __global__ __launch_bounds__(64 * W, 2) void span_wide_kernel(SpanArgs a) {
     };
     // and the rest of q where it could matter
     auto finish_product = [&](f32x16 &x, int tile) {
-        if (!__any(fabsf(sc[(tile - begin) & 3][0][col]) * worst > 1.0f)) return;
+        if (!(__builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(about[(tile - begin) & 3].y)) * worst > 1.0f)) return;
         bool left = true;
 #pragma unroll 1
         for (int round = 1; __any(left); ++round) {
@@ -328,8 +355,9 @@ __global__ __launch_bounds__(64 * W, 2) void span_wide_kernel(SpanArgs a) {
     for (int tile = begin; tile < end; ++tile) {
         const int vb = (tile - begin) & 1, sb = (tile - begin) & 3;
         const int s0 = slot0(tile), behind = stop(tile);
-        const bool odd = __any(!(fabsf(sc[sb][1][col]) < INFINITY));  // an infinite or NaN V scale
-        const int ve = __builtin_amdgcn_readfirstlane(sve[sb]);
+        const int code = __builtin_amdgcn_readfirstlane(about[sb].x);
+        const bool odd = code > kOddTile / 2;
+        const int ve = odd ? code - kOddTile : code;
         f32x16 x;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -367,26 +395,25 @@ __global__ __launch_bounds__(64 * W, 2) void span_wide_kernel(SpanArgs a) {
         top = fmaxf(top, butterfly_partner<32>(top, lane)) * down;
         const int follow = max(-kMostExp, min(kMostExp, ve));
         const float high = ceilf(top) + static_cast<float>(follow);
-        if (__any(high > M + kSlack)) {  // (M = -inf: the first scores)
+        const int beyond = ve - follow;
+        bool apart = false;
+        float up = 0.0f;
+        // (high above M = -inf: the first scores)
+        if (beyond != 0 || __any(high > M + kSlack || (high < M - kDrop && high > -INFINITY))) {
             const float most = fmaxf(M, high);
             const float alpha = M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - most);
             M = most;
-            l *= alpha;
-#pragma unroll
-            for (int i = 0; i < DT; ++i) acc[i] *= alpha;
-        }
-        const int beyond = ve - follow;
-        const bool apart = beyond != 0 || __any(high < M - kDrop && high > -INFINITY);
-        float up = 0.0f;
-        if (apart) {
-            up = high > -INFINITY ? fminf(M - high, static_cast<float>(min(kMostUp, kMostUp + beyond))) : 0.0f;
-            l *= __builtin_amdgcn_exp2f(up);
-            const float grow = __builtin_amdgcn_exp2f(up - static_cast<float>(beyond));
+            apart = beyond != 0 || __any(high < M - kDrop && high > -INFINITY);
+            if (apart && high > -INFINITY) up = fminf(M - high, static_cast<float>(min(kMostUp, kMostUp + beyond)));
+            l *= alpha * __builtin_amdgcn_exp2f(up);
+            const float grow = alpha * __builtin_amdgcn_exp2f(up - static_cast<float>(beyond));
 #pragma unroll
             for (int i = 0; i < DT; ++i) acc[i] *= grow;
         }
         const float lifted = M > -INFINITY ? kLift + up - M : 0.0f;  // nothing attended yet: every power is 0
-        // the next tile's product beside this tile's weights
+        // the next tile's product beside this tile's weights (ahead of the other block's wave: 466 -> 456 us where the
+        // matrix unit is the bound)
+        __builtin_amdgcn_s_setprio(1);
         next = product(tile + 1);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -428,6 +455,7 @@ __global__ __launch_bounds__(64 * W, 2) void span_wide_kernel(SpanArgs a) {
         }
         place_v(rv_next, tile + 1);
         place_k(rk_next, tile + 2);
+        __builtin_amdgcn_s_setprio(0);
         if (apart) {
             l *= __builtin_amdgcn_exp2f(-up);
             const float back = __builtin_amdgcn_exp2f(static_cast<float>(beyond) - up);
@@ -460,33 +488,51 @@ __global__ __launch_bounds__(64 * W, 2) void span_wide_kernel(SpanArgs a) {
     }
 }
 
-template <int HD, int W>
-void launch_wide_hd(const SpanArgs &a, hipStream_t s) {
-    const int64_t tiles = (static_cast<int64_t>(a.count) * a.group + 32 * W - 1) / (32 * W);
-    const dim3 grid(static_cast<unsigned>(tiles * a.splits * a.units * a.kvheads));
-    if (a.positions) hipLaunchKernelGGL((span_wide_kernel<HD, W, true>), grid, dim3(64 * W), 0, s, a);
-    else hipLaunchKernelGGL((span_wide_kernel<HD, W, false>), grid, dim3(64 * W), 0, s, a);
-    ND_HIP(hipGetLastError());
+template <int HD, bool RING>
+__global__ __launch_bounds__(256, 2) void span_wide_kernel(SpanArgs a) {
+    span_wide<HD, RING>(a, blockIdx.x);
+}
+
+// A shared prefix and the units' own keys in one launch: the first `far_blocks` blocks have the prefix.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void span_wide_own_kernel(SpanArgs far, SpanArgs own, int far_blocks) {
+    if (static_cast<int>(blockIdx.x) < far_blocks) span_wide<HD, false>(far, blockIdx.x);
+    else span_own<HD, 4>(own, blockIdx.x - far_blocks);
+}
+
+int64_t wide_blocks(const SpanArgs &a) {
+    const int64_t rows = static_cast<int64_t>(a.count) * a.group, block = 32 * a.groups;
+    return (rows + block - 1) / block * a.splits * a.units * a.kvheads;
 }
 
 template <int HD>
-void launch_wide_w(const SpanArgs &a, int waves, hipStream_t s) {
-    switch (waves) {
-    case 1: launch_wide_hd<HD, 1>(a, s); break;
-    case 2: launch_wide_hd<HD, 2>(a, s); break;
-    case 3: launch_wide_hd<HD, 3>(a, s); break;
-    default: launch_wide_hd<HD, 4>(a, s); break;
-    }
+void launch_wide_hd(const SpanArgs &a, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(wide_blocks(a)));
+    if (a.positions) hipLaunchKernelGGL((span_wide_kernel<HD, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((span_wide_kernel<HD, false>), grid, dim3(256), 0, s, a);
+    ND_HIP(hipGetLastError());
 }
 
 }  // namespace
 
-void launch_span_wide(const SpanArgs &a, int head_dim, int waves, hipStream_t s) {
+void launch_span_wide(const SpanArgs &a, int head_dim, hipStream_t s) {
     switch (head_dim) {
-    case 32: launch_wide_w<32>(a, waves, s); break;
-    case 64: launch_wide_w<64>(a, waves, s); break;
-    default: launch_wide_w<128>(a, waves, s); break;
+    case 32: launch_wide_hd<32>(a, s); break;
+    case 64: launch_wide_hd<64>(a, s); break;
+    default: launch_wide_hd<128>(a, s); break;
     }
+}
+
+void launch_span_wide_own(const SpanArgs &far, const SpanArgs &own, int head_dim, hipStream_t s) {
+    const int64_t far_blocks = wide_blocks(far);
+    const dim3 grid(static_cast<unsigned>(far_blocks + static_cast<int64_t>(own.splits) * own.kvheads * own.units));
+    const int n = static_cast<int>(far_blocks);
+    switch (head_dim) {
+    case 32: hipLaunchKernelGGL((span_wide_own_kernel<32>), grid, dim3(256), 0, s, far, own, n); break;
+    case 64: hipLaunchKernelGGL((span_wide_own_kernel<64>), grid, dim3(256), 0, s, far, own, n); break;
+    default: hipLaunchKernelGGL((span_wide_own_kernel<128>), grid, dim3(256), 0, s, far, own, n); break;
+    }
+    ND_HIP(hipGetLastError());
 }
 
 }  // namespace nd

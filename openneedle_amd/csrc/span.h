@@ -79,9 +79,12 @@ struct EvictArgs {
     float *new_weights;    // may be `weights`
     const int *lengths;
     int *new_lengths;      // may be `lengths`
-    int *kept, *counts;    // counts[seqs]: min(n, keep)
+    int *kept;             // null only for one launch
+    int *counts;           // [seqs], two launches: min(n, keep)
     int seqs, kvheads, head_dim, keep, sinks, recent;
 };
+// whether launch_evict needs `kept` and `counts` between two launches
+bool evict_takes_two(const EvictArgs &a);
 void launch_evict(const EvictArgs &a, hipStream_t s);
 
 }  // namespace nd

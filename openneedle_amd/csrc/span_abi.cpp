@@ -266,9 +266,11 @@ int needle2_gpu_kv_evict(void *h, int layer, const float *d_weights, const int *
         a.keep = keep;
         a.sinks = sinks;
         a.recent = recent;
-        const size_t rows = size_t(kv.seqs) * kv.kvheads * keep;
-        a.counts = kv.kept.reserve(kv.seqs + (d_kept ? 0 : rows));
-        a.kept = d_kept ? d_kept : a.counts + kv.seqs;
+        a.kept = d_kept;
+        if (evict_takes_two(a)) {
+            a.counts = kv.kept.reserve(kv.seqs + (d_kept ? 0 : size_t(kv.seqs) * kv.kvheads * keep));
+            if (!d_kept) a.kept = a.counts + kv.seqs;
+        }
         launch_evict(a, static_cast<hipStream_t>(stream));
     });
 }

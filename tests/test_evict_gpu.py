@@ -160,3 +160,17 @@ def test_refusals_change_nothing():
     synchronize()
     for a, b in zip(kv.read(0, 0, 32), rows[0, 0]):
         np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("keep", [12288, 12289])
+def test_long_lists(hd, keep):
+    """Around the longest list of kept slots that one launch holds, more slots than a block has in registers."""
+    rng = np.random.default_rng(keep)
+    cap = 20001
+    kv, rows = filled(rng, 1, cap, 1, hd)
+    w = weights(rng, 1, 1, cap)
+    for kept in (True, False):
+        check(kv, rows, w, [cap], keep, 7, 1000, run(kv, w, [cap], keep, 7, 1000, kept=kept))
+        kv, rows = filled(rng, 1, cap, 1, hd)

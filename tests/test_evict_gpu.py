@@ -25,9 +25,23 @@ def filled(rng, seqs, cap, kvh, hd, layers=1):
         for s in range(seqs):
             k, v = (rng.integers(-127, 128, (cap, kvh, hd)).astype(np.int8) for _ in "kv")
             ks, vs = (rng.uniform(0.01, 0.03, (cap, kvh)).astype(np.float32) for _ in "kv")
-            kv.load(layer, s, k, v, ks, vs)
             rows[layer, s] = (k, v, ks, vs)
+        write_rows(kv, layer, [np.stack([rows[layer, s][i] for s in range(seqs)]) for i in range(4)])
     return kv, rows
+
+
+def write_rows(kv, layer, rows):
+    """(k, v, ks, vs) [seqs][slots][kvheads]... of a whole layer into the cache, through its device memory."""
+    for at, a in zip(kv.device_rows(layer), rows):
+        at.upload(np.swapaxes(a, 1, 2))
+
+
+def read_rows(kv, layer):
+    """The same back."""
+    shape = (kv.seqs, kv.kvheads, kv.capacity)
+    shapes = (shape + (kv.head_dim,),) * 2 + (shape,) * 2
+    kinds = (np.int8, np.int8, np.float32, np.float32)
+    return [np.swapaxes(at.to_host(k, n), 1, 2) for at, k, n in zip(kv.device_rows(layer), kinds, shapes)]
 
 
 def run(kv, w, lengths, keep, sinks, recent, layer=0, alias=False, kept=True, stream=None):
@@ -48,6 +62,7 @@ def run(kv, w, lengths, keep, sinks, recent, layer=0, alias=False, kept=True, st
 def check(kv, rows, w, lengths, keep, sinks, recent, got, layer=0):
     new_w, new_n, kept = got
     cap = kv.capacity
+    now = read_rows(kv, layer)
     for s in range(kv.seqs):
         n = min(max(int(lengths[s]), 0), cap)
         left = min(n, keep)
@@ -61,8 +76,8 @@ def check(kv, rows, w, lengths, keep, sinks, recent, got, layer=0):
             np.testing.assert_array_equal(new_w[s, h], np.concatenate([w[s, h, slots], np.zeros(cap - left, np.float32)]))
             for a, b in zip(after, rows[layer, s]):
                 a[:left, h] = b[slots, h]
-        for a, b in zip(kv.read(layer, s, cap), after):
-            np.testing.assert_array_equal(a, b, err_msg=f"sequence {s}")
+        for a, b in zip(now, after):
+            np.testing.assert_array_equal(a[s], b, err_msg=f"sequence {s}")
 
 
 def weights(rng, seqs, kvh, cap):
@@ -124,9 +139,9 @@ def test_in_place_layers_and_streams(kept):
     got = run(kv, w, [700, 650], 333, 4, 32, layer=1, alias=True, kept=kept, stream=stream)
     check(kv, rows, w, [700, 650], 333, 4, 32, got, layer=1)
     for layer in (0, 2):
-        for s in range(2):
-            for a, b in zip(kv.read(layer, s, cap), rows[layer, s]):
-                np.testing.assert_array_equal(a, b)
+        for i, a in enumerate(read_rows(kv, layer)):
+            for s in range(2):
+                np.testing.assert_array_equal(a[s], rows[layer, s][i])
 
 
 @pytest.mark.gpu
@@ -139,7 +154,8 @@ def test_many_sequences_and_a_second_cut():
     lengths = rng.integers(0, cap + 1, seqs).astype(np.int32)
     got = run(kv, w, lengths, 257, 4, 30)
     check(kv, rows, w, lengths, 257, 4, 30, got)
-    rows = {(0, s): kv.read(0, s, cap) for s in range(seqs)}
+    now = read_rows(kv, 0)
+    rows = {(0, s): tuple(a[s] for a in now) for s in range(seqs)}
     again = run(kv, got[0], got[1], 100, 4, 30)
     check(kv, rows, got[0], got[1], 100, 4, 30, again)
 

@@ -14,7 +14,7 @@ import pytest
 import oracle
 from openneedle_amd.device import DeviceArray, Graph, Stream, synchronize
 from openneedle_amd.kv import KVCache
-from tests.test_evict_gpu import kept_slots
+from tests.test_evict_gpu import kept_slots, read_rows, write_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -31,8 +31,7 @@ class Rows:
         self.push()
 
     def push(self):
-        for s in range(self.k.shape[0]):
-            self.kv.load(self.layer, s, self.k[s], self.v[s], self.ks[s], self.vs[s])
+        write_rows(self.kv, self.layer, (self.k, self.v, self.ks, self.vs))
 
     def put(self, s, slot, k, v):
         for codes, scales, rows in ((self.k, self.ks, k), (self.v, self.vs, v)):
@@ -46,9 +45,8 @@ class Rows:
 
     def same(self):
         """The cache holds exactly these rows."""
-        for s in range(self.k.shape[0]):
-            for a, b in zip(self.kv.read(self.layer, s, self.k.shape[1]), (self.k[s], self.v[s], self.ks[s], self.vs[s])):
-                np.testing.assert_array_equal(a, b, err_msg=f"sequence {s}: rows")
+        for a, b in zip(read_rows(self.kv, self.layer), (self.k, self.v, self.ks, self.vs)):
+            np.testing.assert_array_equal(a, b)
 
 
 def attend(q, k, v):
@@ -530,7 +528,7 @@ def test_graph_replays_match_eager(count):
 
     def results(d):
         return [d[k].to_host(np.uint32, d[k].nbytes // 4) for k in ("o", "o1", "o2", "w", "w2", "n2")] + \
-            [a for name in ("ring", "own") for s in range(seqs) for a in d[name].kv.read(0, s, d[name].k.shape[1])]
+            [a for name in ("ring", "own") for a in read_rows(d[name].kv, 0)]
 
     stream = Stream()
     graphed, eager = state(1), state(1)
@@ -606,9 +604,11 @@ def test_refusals_change_nothing():
 def test_device_rows():
     rng = np.random.default_rng(41)
     r = Rows(rng, 2, 9, 3, 32, layers=2, layer=1)
-    k, v, ks, vs = r.kv.device_rows(1)
-    for at, a in ((k, r.k), (v, r.v), (ks, r.ks), (vs, r.vs)):
-        want = np.swapaxes(a, 1, 2)
-        np.testing.assert_array_equal(at.to_host(a.dtype, want.shape), want)
+    for s in range(2):  # written through device_rows, read as host rows
+        for a, b in zip(r.kv.read(1, s, 9), (r.k, r.v, r.ks, r.vs)):
+            np.testing.assert_array_equal(a, b[s])
+        r.kv.load(1, s, r.k[1 - s], r.v[1 - s], r.ks[1 - s], r.vs[1 - s])
+    for a, b in zip(read_rows(r.kv, 1), (r.k, r.v, r.ks, r.vs)):
+        np.testing.assert_array_equal(a, b[::-1])
     with pytest.raises(RuntimeError, match="layer"):
         r.kv.device_rows(2)

@@ -30,7 +30,8 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
 
     const int t = threadIdx.x, lane = t & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int piece = bx % a.splits, tile0 = bx / a.splits;
+    const int tiles_of_rows = (a.count * a.group + kSpanRows - 1) / kSpanRows;
+    const int tile0 = bx % tiles_of_rows, piece = bx / tiles_of_rows;
     const int rows = a.count * a.group;
     const int row = tile0 * kSpanRows + col;
     const int last_row = min(rows, (tile0 + 1) * kSpanRows) - 1;
@@ -351,11 +352,12 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
     }
 }
 
-// Block `b` of the launch of a's units, each with its own keys.
-template <int HD, int NW>
-__device__ __forceinline__ void span_own(const SpanArgs &a, int b) {
-    const int rest = b / a.splits;
-    span_rows<HD, NW, false>(a, b % a.splits, rest % a.kvheads, rest / a.kvheads);
+// Block `b` of a launch of all units, kv heads, row tiles and pieces. The pieces are slowest: those behind the end of a
+// short sequence come last, and the others spread over the compute units.
+template <int HD, int NW, bool RING>
+__device__ __forceinline__ void span_block(const SpanArgs &a, int b) {
+    const int rest = b / a.kvheads;
+    span_rows<HD, NW, RING>(a, rest / a.units, b % a.kvheads, rest % a.units);
 }
 
 }  // namespace

@@ -298,11 +298,12 @@ int needle2_gpu_kv_export(void *kv, int layer, int seq, int8_t *k, int8_t *v, fl
  * The reference attends one sequence's window through a slot list
  * (needle2/csrc/engine.cpp:898-911) and neither shares a prefix between
  * sequences nor drops slots; these serve a batch. heads: a multiple of kvheads,
- * 1 to 16 query heads per kv head. Nothing is read on the host, so every call
- * can be captured once it has run with the same sizes (its scratch belongs to
- * the handle, is never moved while the handle lives, and is not for two calls
- * at once). The handle must have been made on the current device. All return
- * 0 / -1 (message in needle2_gpu_error); a refused call does nothing. */
+ * 1 to 16 query heads per kv head, at most 2^22 over the batch. Nothing is
+ * read on the host, so every call can be captured once it has run with the
+ * same sizes (its scratch belongs to the handle, is never moved while the
+ * handle lives, and is not for two calls at once). The handle must have been
+ * made on the current device. All return 0 / -1 (message in
+ * needle2_gpu_error); a refused call does nothing. */
 
 /* Attention of `count` consecutive new tokens per sequence over a window with
  * pinned first positions. d_q, d_out: device fp32 [seqs][count][heads][head_dim].
@@ -313,7 +314,7 @@ int needle2_gpu_kv_export(void *kv, int layer, int seq, int8_t *k, int8_t *v, fl
  * stored already), then token i attends every position up to its own that is
  * below sinks or among the last `window`. A token at a negative position (left
  * padding, an idle sequence) is not stored and its output is zero. Needs
- * sinks + window + count - 1 <= capacity, at most 2^26 query rows. */
+ * sinks + window + count - 1 <= capacity, at most 2^25 query rows. */
 int needle2_gpu_attention_window(void *kv, int layer, const float *d_q, float *d_out, int heads, int count,
                                  const int *d_positions, int sinks, int window, const float *d_new_k,
                                  const float *d_new_v, void *stream);
@@ -329,7 +330,9 @@ int needle2_gpu_attention_shared(void *kv, int layer, void *prefix, int prefix_s
 /* One decode step over slots [0, n) as above that also adds to
  * d_weights[s][kvhead][slot] (device fp32 [seqs][kvheads][capacity]) the slot's
  * softmax weights, summed over the kv head's query heads; entries from n on are
- * left as they are. A head without a softmax (a non-finite query) adds nothing. */
+ * left as they are. A head without a softmax (a non-finite query) adds nothing.
+ * The handle's scratch for it is 4 bytes per query head, sequence and slot of
+ * its capacity. */
 int needle2_gpu_attention_weights(void *kv, int layer, const float *d_q, float *d_out, float *d_weights, int heads,
                                   int length, const int *d_lengths, const float *d_new_k, const float *d_new_v,
                                   void *stream);

@@ -3,20 +3,22 @@
 
 #include "abi_internal.h"
 
+#include <algorithm>
 #include <memory>
 #include <vector>
 
 namespace nd {
 
 // Device scratch of a handle that only grows and never moves under a captured graph: what it outgrows stays allocated
-// until the handle is destroyed, so a graph captured with the smaller buffer may still be replayed.
+// until the handle is destroyed, so a graph captured with the smaller buffer may still be replayed. It at least doubles,
+// so that all of it together is at most twice the last.
 template <class T>
 struct KeptBuf {
     std::vector<std::unique_ptr<DevBuf<T>>> bufs;
     T *reserve(size_t count) {
         if (bufs.empty() || bufs.back()->n < count) {
             auto b = std::make_unique<DevBuf<T>>();
-            b->reserve(count);
+            b->reserve(bufs.empty() ? count : std::max(count, 2 * bufs.back()->n));
             bufs.push_back(std::move(b));
         }
         return bufs.back()->p;

@@ -239,7 +239,8 @@ int needle2_gpu_attention_weights(void *h, int layer, const float *d_q, float *d
         a.splits_total = a.splits;
         reserve_records(kv, a, int64_t(kv.seqs) * heads);  // for one piece too: the weights need the final sums
         a.score_stride = std::max(1, span_tiles(length)) * kSpanTile;
-        a.scores = kv.scores.reserve(size_t(kv.seqs) * heads * a.score_stride);
+        // for the whole capacity: a length that grows with every step must not grow the scratch with it
+        a.scores = kv.scores.reserve(size_t(kv.seqs) * heads * span_tiles(kv.capacity) * kSpanTile);
         SpanRecordArgs r{a, d_weights};
         launch_span(a, kv.head_dim, s);
         launch_span_record(r, kv.head_dim, s);

@@ -8,13 +8,14 @@
 namespace nd {
 
 constexpr int kSpanMaxGroup = 16;  // query heads per kv head
-constexpr int kMaxGrid = 65535;    // blocks in a grid's second and third dimension
+constexpr int kMaxGrid = 65535;    // blocks in a grid's second and third dimension (and less than 2^32 threads in the first)
 
 // seqs, kvheads: the cache's.
 inline const char *check_heads(int seqs, int kvheads, int heads) {
     if (heads <= 0 || heads % kvheads) return "attention: heads must be a multiple of kvheads";
     if (heads / kvheads > kSpanMaxGroup) return "attention: at most 16 query heads per kv head";
     if (seqs > kMaxGrid || kvheads > kMaxGrid) return "attention: at most 65535 sequences and kv heads";
+    if (int64_t(seqs) * heads > (int64_t(1) << 22)) return "attention: more than 2^22 query heads in the batch";
     return nullptr;
 }
 
@@ -25,7 +26,7 @@ inline const char *check_window(int capacity, int seqs, int kvheads, int heads, 
     if (window < 1) return "attention: window must be >= 1";
     if (int64_t(sinks) + window + (count > 0 ? count : 1) - 1 > capacity)
         return "attention: sinks + window + count - 1 exceeds the cache capacity";
-    if (int64_t(seqs) * count * heads > (int64_t(1) << 26)) return "attention: more than 2^26 query rows";
+    if (int64_t(seqs) * count * heads > (int64_t(1) << 25)) return "attention: more than 2^25 query rows";
     return nullptr;
 }
 

@@ -108,7 +108,8 @@ def test_argument_rules(host):
                        ((20, 2, 2, 34, 1, 4, 16), b"16 query heads"), ((20, 2, 2, 4, -1, 4, 16), b"count"),
                        ((20, 2, 2, 4, 1, -1, 16), b"sinks"), ((20, 2, 2, 4, 1, 4, 0), b"window"),
                        ((20, 2, 2, 4, 2, 4, 16), b"capacity"), ((20, 2, 2, 4, 1, 2 ** 31 - 1, 2 ** 31 - 1), b"capacity"),
-                       ((2 ** 30, 64, 2, 32, 2 ** 20, 4, 16), b"rows"), ((20, 70000, 1, 1, 1, 4, 16), b"65535")]:
+                       ((2 ** 30, 64, 2, 32, 2 ** 20, 4, 16), b"rows"), ((20, 70000, 1, 1, 1, 4, 16), b"65535"),
+                       ((2 ** 25, 64, 2, 32, 2 ** 14 + 1, 4, 16), b"2^25"), ((20, 2 ** 15, 2 ** 4, 2 ** 8, 1, 4, 16), b"2^22")]:
         assert word in host.window_rule(*args), args
     assert host.length_rule(20, 2, 2, 4, 0) is None and host.length_rule(20, 2, 2, 4, 20) is None
     assert b"length" in host.length_rule(20, 2, 2, 4, 21) and b"length" in host.length_rule(20, 2, 2, 4, -1)

@@ -559,6 +559,36 @@ def test_graph_replays_match_eager(count):
     g.close()
 
 
+def test_unaligned_buffers_and_growing_lengths():
+    """Buffers that start at any float; a length that grows with every step (the scratch does not grow with it)."""
+    rng = np.random.default_rng(33)
+    r = Rows(rng, 2, 300, 2, 64)
+    q = rng.normal(size=(2, 4, 64)).astype(np.float32)
+    record = np.zeros((2, 2, 300), np.float32)
+    big = [DeviceArray(n + 16) for n in (q.nbytes, q.nbytes, record.nbytes, q.nbytes // 2, q.nbytes // 2)]
+    for off in (4, 8, 12):
+        d_q, d_o, d_w, d_k, d_v = (b.view(off, b.nbytes - 16) for b in big)
+        for length in range(10, 301, 29):
+            new = tuple(rng.normal(size=(2, 2, 64)).astype(np.float32) for _ in "kv")
+            for d, a in zip((d_q, d_w, d_k, d_v), (q, record, *new)):
+                d.upload(a)
+            r.kv.attention_weights(0, d_q, d_o, d_w, 4, length, new=(d_k, d_v))
+            synchronize()
+            for s in range(2):
+                r.put(s, length - 1, new[0][s], new[1][s])
+            got_w = d_w.to_host(np.float32, record.shape)
+            check_weights(r, q, record, [length] * 2, d_o.to_host(np.float32, q.shape), got_w)
+        d_n = upload([299, 299], np.int32)
+        many, d_m = rng.normal(size=(2, 40, 4, 64)).astype(np.float32), DeviceArray(2 * 40 * 4 * 64 * 4 + 16)
+        d_p, d_r = d_m.view(off, d_m.nbytes - 16), DeviceArray(d_m.nbytes)
+        d_p.upload(many)
+        d_r = d_r.view(off, d_m.nbytes - 16)
+        r.kv.attention_window(0, d_p, d_r, 4, 40, d_n, 4, 200)
+        synchronize()
+        check_window(r, many, [299, 299], 4, 200, d_r.to_host(np.float32, many.shape), tokens=(0, 17, 39))
+    r.same()
+
+
 def test_same_results_every_time():
     rng = np.random.default_rng(30)
     r = Rows(rng, 2, 3000, 2, 128)

@@ -116,8 +116,13 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
     constexpr int KS = HD / 16;                     // steps of the score product's depth
     constexpr int DT = HD / 32;                     // results of 32 dimensions
     constexpr int T = 256;
-    constexpr int kChunks = 2 * HD;                 // of a tile's K codes, 16 bytes each; and pieces of V, 4 keys x 4 dimensions
-    constexpr int C = (kChunks + T - 1) / T;        // of each per thread
+    // A tile's K codes are 2 HD chunks of 16 bytes, its V codes as many pieces of 4 keys x 4 dimensions: one of each a
+    // thread (HD = 128), or K's on the first waves and V's on the next.
+    constexpr int kChunks = 2 * HD;
+    constexpr bool kBoth = kChunks == T;
+    constexpr int kRoleWaves = kChunks / 64;
+    constexpr int kScaleWave = HD == 32 ? 2 : 0;    // it brings the scales too
+    static_assert(kBoth || 2 * kChunks <= T, "roles of the waves");
     __shared__ u32x4 kf[2][KS][kFrag];
     __shared__ u32x4 vf[2][2][DT][kFrag];
     __shared__ __attribute__((aligned(16))) float sc[4][2][kWideTile];  // K (times scale) and V scales, by tile modulo 4
@@ -164,41 +169,38 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
 
     // Codes on their way to LDS: K as 16 dimensions of a key, V as 4 dimensions of 4 keys. Loads past the cache's rows
     // read zero.
+    constexpr uint32_t kNone = 0x80000000u;  // past every buffer: no request
+    const bool k_role = kBoth || wave < kRoleWaves, v_role = kBoth || (wave >= kRoleWaves && wave < 2 * kRoleWaves);
+    const int kc = t, vc = kBoth ? t : t - kChunks;  // chunk, piece
+    const int v_keys = vc / (HD / 4), v_dims = vc % (HD / 4);
     struct RawK {
-        u32x4 k[C];
+        u32x4 k;
         float s[2];  // K and V scale of key `col`
     };
     struct RawV {
-        uint32_t v[C][4];
+        uint32_t v[4];
     };
     auto fetch_k = [&](RawK &r, int tile) {
         const uint32_t s0 = static_cast<uint32_t>(slot0(tile));
-#pragma unroll
-        for (int i = 0; i < C; ++i) r.k[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, s0 * HD + (t + i * T) * 16, 0, 0);
-        const uint32_t at = (s0 + col) * 4u;
+        r.k = __builtin_amdgcn_raw_buffer_load_b128(rk, k_role ? s0 * HD + kc * 16 : kNone, 0, 0);
+        const uint32_t at = wave == kScaleWave ? (s0 + col) * 4u : kNone;
         r.s[0] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rks, at, 0, 0));
         r.s[1] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rvs, at, 0, 0));
     };
     auto fetch_v = [&](RawV &r, int tile) {
         const uint32_t s0 = static_cast<uint32_t>(slot0(tile));
+        const uint32_t at = v_role ? (s0 + 4 * v_keys) * HD + v_dims * 4 : kNone;
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int c = t + i * T, keys = c / (HD / 4), dims = c % (HD / 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                r.v[i][j] = __builtin_amdgcn_raw_buffer_load_b32(rv, (s0 + 4 * keys + j) * HD + dims * 4, 0, 0);
-        }
+        for (int j = 0; j < 4; ++j) r.v[j] = __builtin_amdgcn_raw_buffer_load_b32(rv, at + j * HD, 0, 0);
     };
     auto place_k = [&](const RawK &r, int tile) {
         const int buf = (tile - begin) & 1, sb = (tile - begin) & 3;
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int c = t + i * T, key = c / KS, step = c % KS;
-            if (kChunks % T != 0 && c >= kChunks) break;
-            kf[buf][step][frag_lane(key, 0)] = widen_half(r.k[i].x, r.k[i].y);
-            kf[buf][step][frag_lane(key, 1)] = widen_half(r.k[i].z, r.k[i].w);
+        if (k_role) {
+            const int key = kc / KS, step = kc % KS;
+            kf[buf][step][frag_lane(key, 0)] = widen_half(r.k.x, r.k.y);
+            kf[buf][step][frag_lane(key, 1)] = widen_half(r.k.z, r.k.w);
         }
-        if (wave == 0) {
+        if (wave == kScaleWave) {
             const bool in = slot0(tile) + col < stop(tile);
             const float ks = in ? r.s[0] * a.scale : 0.0f, vs = in ? r.s[1] : 0.0f;
             sc[sb][half][col] = half ? vs : ks;
@@ -211,20 +213,17 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
         }
     };
     auto place_v = [&](const RawV &r, int tile) {
+        if (!v_role) return;
         const int buf = (tile - begin) & 1;
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int c = t + i * T, keys = c / (HD / 4), dims = c % (HD / 4);  // 4 keys: half and quarter of a step's depth
-            if (kChunks % T != 0 && c >= kChunks) break;
+        for (int b = 0; b < 4; ++b) {
+            float f[4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                float f[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) f[j] = code(r.v[i][j], b);
-                const int d = dims * 4 + b;
-                u32x2 *to = reinterpret_cast<u32x2 *>(&vf[buf][keys / 4][d % DT][frag_lane(d / DT, keys & 1)]);
-                to[(keys >> 1) & 1] = u32x2{half_pair(f[0], f[1]), half_pair(f[2], f[3])};
-            }
+            for (int j = 0; j < 4; ++j) f[j] = code(r.v[j], b);
+            const int d = v_dims * 4 + b;
+            // 4 keys: half and quarter of a step's depth
+            u32x2 *to = reinterpret_cast<u32x2 *>(&vf[buf][v_keys / 4][d % DT][frag_lane(d / DT, v_keys & 1)]);
+            to[(v_keys >> 1) & 1] = u32x2{half_pair(f[0], f[1]), half_pair(f[2], f[3])};
         }
     };
 

@@ -43,12 +43,12 @@ struct SpanArgs {
 };
 
 // New tokens [seqs][count][kvheads][head_dim] into ring slots: token i of sequence s at position positions[s] + i
-// (negative positions are not stored); or, without positions, into slot lengths[s] - 1 (count 1).
+// (negative positions are not stored).
 struct SpanStoreArgs {
     SpanCache c;
     const float *k, *v;
-    const int *positions, *lengths;
-    int seqs, count, kvheads, head_dim, length, sinks;
+    const int *positions;
+    int seqs, count, kvheads, head_dim, sinks;
 };
 
 // record[unit][kvh][slot] += the softmax weights of the kv head's rows, and the rows' outputs from their records.

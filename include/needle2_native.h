@@ -240,7 +240,8 @@ int needle2_gpu_device_info(char *buf, int len);         /* "name;arch;cus;hbm_b
 /* HIP graphs (no counterpart in the reference, which has no device): capture
  * what is issued to `stream` between begin and end, instantiate, replay with
  * one launch. Entry points used inside must have run once before the capture
- * and must not read host memory: plan_run, attention, kv_store_device. */
+ * and must not read host memory: plan_run, attention (all forms),
+ * kv_store_device, kv_evict. */
 int needle2_gpu_graph_begin(void *stream);
 void *needle2_gpu_graph_end(void *stream);                /* instantiated graph, or NULL */
 int needle2_gpu_graph_launch(void *graph, void *stream);

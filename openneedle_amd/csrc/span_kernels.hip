@@ -85,7 +85,7 @@ __device__ __forceinline__ float2 join_sums(const SpanArgs &a, size_t row, int l
 
 // Rows row0 .. row0 + count - 1 from their records, by a block of 256: G groups of HD / 4 lanes share a row's records
 // (every G-th each), whose loads do not wait for each other; 256 / (G * HD / 4) rows at a time. The sums' order depends
-// on the number of records only.
+// on the number of records only. Latency bounds it: 64 x 32 rows of 128 values 5 us, a long prefix's many records 7.
 constexpr int kJoinMax = 1024;  // records of a row
 template <int HD, int G>
 __device__ __forceinline__ void join_rows(const SpanArgs &a, size_t row0, int count) {

@@ -14,7 +14,10 @@ __device__ __forceinline__ f32x4 mfma(const u32x4 &a, const u32x4 &b, const f32x
 
 // Block (piece and row tile, kv head, unit): up to 16 query rows (the columns of both products' results), NW waves with
 // every NW-th tile of 64 keys each, joined at the end. Eight waves where there is at most one block per compute unit: a
-// block's rounds then bound the launch (one conversation of 272 keys 8.7 -> 6.8 us, 35 blocks of 1006 keys of 32 values 13.8 -> 11.0).
+// block's rounds then bound the launch (one conversation of 272 keys 8.7 -> 6.8 us, 35 blocks of 1006 keys of
+// 32 values 13.8 -> 11.0). With many blocks the cache's rows bound it, read once, each lane its operands' bytes straight
+// from memory: 64 sequences x 8 kv heads x 4100 keys of 128 values, 101 us (5.5 TB/s). Three terms cost matrix work that
+// stays below that time at 16 rows a block.
 //   Scores: operand A is 16 keys' codes, operand B the rows' q. Lane l holds row l % 16 and keys 16 t + 4 (l / 16) + i.
 //   Values: operand B is p * vs straight from those registers (the contraction runs over the keys in their order:
 //   depth 8 (l / 16) + j is key 32 u + 4 (l / 16) + j, and from j = 4 on 32 u + 16 + 4 (l / 16) + j - 4), operand A the V

@@ -7,6 +7,10 @@
 //   2^-24 of its size) the tile's scores get the rest of q in further terms, until nothing is left.
 //   p * vs is scaled so that the largest of a row's 32 in a tile is at least 2^2: what the terms leave is below 2^-27 of
 //   it, where an fp32 sum of the 32 rounds by 2^-24 of its largest term.
+// 6 x 999 tokens, 32 heads of 128 values, window 2048: 428 us, 1.0 PFLOP/s of matrix work (a large bfloat16 product of the
+// library reaches 1.2). The matrix unit is busy 47% of the cycles; the rest is the softmax and the making of terms, 258
+// vector instructions a wave and tile next to its 32 matrix instructions. Rows of 64: 362 us. A third block a
+// compute unit spills.
 #include "span_rows.h"
 
 namespace nd {

@@ -303,8 +303,9 @@ int needle2_gpu_kv_export(void *kv, int layer, int seq, int8_t *k, int8_t *v, fl
  * read on the host, so every call can be captured once it has run with the
  * same sizes (its scratch belongs to the handle, is never moved while the
  * handle lives, and is not for two calls at once). The handle must have been
- * made on the current device. All return 0 / -1 (message in
- * needle2_gpu_error); a refused call does nothing. */
+ * made on the current device. A head without a softmax (no slot to attend, a
+ * non-finite query) yields zeros, as in needle2_gpu_attention. All return
+ * 0 / -1 (message in needle2_gpu_error); a refused call does nothing. */
 
 /* Attention of `count` consecutive new tokens per sequence over a window with
  * pinned first positions. d_q, d_out: device fp32 [seqs][count][heads][head_dim].

@@ -5,6 +5,7 @@
 #include "common.h"
 #include "span_check.h"
 #include "span_geom.h"
+#include "span_plan.h"
 
 namespace nd {
 
@@ -56,8 +57,6 @@ struct SpanRecordArgs {
     SpanArgs a;
     float *record;         // [units][kvheads][capacity]
 };
-
-constexpr int kSpanRows = 16;      // query rows of a block
 
 void launch_span_store(const SpanStoreArgs &a, hipStream_t s);
 // Blocks of 16 query rows; and of 32 * groups, whose keys are turned into operands once for them all.

@@ -41,69 +41,11 @@ static SpanArgs span_args(KvHandle &kv, const SpanCache &c, const float *d_q, fl
     return a;
 }
 
-// How a launch is cut, by estimates (us) from measurements at 256 compute units. A round of a 16-row block (a tile of 64
-// keys per wave) takes 1.2 / 1.25 / 1.85 for rows of 32 / 64 / 128 values with at most one block per unit, of four or
-// eight waves, and 1.6 / 2.4 / 4.1 with two of four; a tile of a wide block (32 keys) 1.15 / 1.15 / 1.2 and
-// 1.5 / 1.7 / 2.3. Blocks start and end in 5 (eight waves 5.8, wide 6), a join launch takes 3.5, records are written and
-// read at 3 TB/s, a piece of a 16-row block costs 0.5 more, and a unit takes its keys at 20 GB/s.
-struct Rate {
-    int waves;               // of a block
-    int tiles;               // of a round
-    double start, one, two;  // us a block, and a round with one block per compute unit and with two (0: never two)
-};
-struct Cut {
-    double us = 0;
-    int splits = 1, per = 1, waves = 4;
-};
-
-// The cheapest cut of blocks of `tiles` tiles and `bytes` each, `blocks` of them without pieces.
-static void best_cut(Cut &best, int64_t blocks, int tiles, double bytes, const Rate &r, double record, double join) {
-    const int cus = device_cus(), room = r.two > 0 ? 2 * cus : cus;
-    const int rounds = (tiles + r.tiles - 1) / r.tiles;
-    const int most = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rounds, room / blocks)));
-    for (int s = 1;; s = std::min(most, s < 4 ? s + 1 : s + s / 3)) {
-        const int64_t n = s * blocks;
-        const int per = (rounds + s - 1) / s;
-        const bool one = n <= cus;
-        if (!one && r.two == 0) return;
-        const double flights = one ? 1 : double((n + room - 1) / room);
-        const double stream = blocks * bytes / (double(std::min<int64_t>(n, cus)) * 2e4);
-        const double us = std::max(stream, flights * (r.start + per * (one ? r.one : r.two))) + (s > 1 ? join : 0) + s * record;
-        if (best.us == 0 || us < best.us) best = Cut{us, (rounds + per - 1) / per, per * r.tiles, r.waves};
-        if (s >= most) return;
-    }
-}
-
-// Cuts `a`; true: for the wide kernel. keys: at most so many per row tile of 16 (wide: of 128) rows, in `runs` runs;
-// joined: a join follows in any case.
-static bool plan(SpanArgs &a, int head_dim, int keys, int wide_keys, int runs, bool joined, bool may_wide) {
-    static const Rate kFour[3] = {{4, 4, 5, 1.2, 1.6}, {4, 4, 5, 1.25, 2.4}, {4, 4, 5, 1.85, 4.1}};
-    static const Rate kEight[3] = {{8, 8, 5.8, 1.2, 0}, {8, 8, 5.8, 1.25, 0}, {8, 8, 5.8, 1.85, 0}};
-    static const Rate kWide[3] = {{4, 1, 6, 1.15, 1.5}, {4, 1, 6, 1.15, 1.7}, {4, 1, 6, 1.2, 2.3}};
-    const int h = head_dim == 32 ? 0 : head_dim == 64 ? 1 : 2;
-    const int64_t rows = int64_t(a.count) * a.group, units = int64_t(a.units) * a.kvheads;
-    const double record = double(rows) * units * head_dim * 8 / 3e6, join = joined ? 0 : 3.5;
-    const int64_t blocks = (rows + kSpanRows - 1) / kSpanRows * units;
-    const int tiles = std::max(1, span_tiles(keys) + runs - 1);
-    const double row = 2.0 * (head_dim + 4);
-    Cut c;
-    best_cut(c, blocks, tiles, keys * row, kFour[h], record + 0.5, join);
-    best_cut(c, blocks, tiles, keys * row, kEight[h], record + 0.5, join);
-    bool wide = false;
-    if (may_wide && rows > kSpanRows) {
-        const int64_t row_blocks = (rows + 127) / 128;
-        Cut w;
-        best_cut(w, row_blocks * units, std::max(1, wide_tiles(wide_keys) + runs - 1), wide_keys * row, kWide[h], record, join);
-        wide = w.us < c.us;
-        if (wide) {
-            c = w;
-            a.groups = a.positions ? 4 : int(((rows + 31) / 32 + row_blocks - 1) / row_blocks);
-        }
-    }
+static void use(SpanArgs &a, const SpanCut &c) {
     a.splits = c.splits;
     a.per = c.per;
     a.waves = c.waves;
-    return wide;
+    a.groups = c.groups;
 }
 
 static void launch(const SpanArgs &a, bool wide, int head_dim, hipStream_t s) {
@@ -144,12 +86,8 @@ int needle2_gpu_attention_window(void *h, int layer, const float *d_q, float *d_
         a.positions = d_positions;
         a.sinks = sinks;
         a.window = window;
-        // keys of a block: its tokens' windows
-        auto keys = [&](int rows) {
-            const int64_t tokens = (rows + a.group - 1) / a.group + 1;
-            return int(std::min<int64_t>(sinks + int64_t(window) + std::min<int64_t>(count, tokens) - 1, kv.capacity));
-        };
-        const bool wide = plan(a, kv.head_dim, keys(kSpanRows), keys(128), 2, false, true);
+        const SpanCut cut = cut_window(device_cus(), kv.head_dim, kv.capacity, kv.seqs, kv.kvheads, heads, count, sinks, window);
+        use(a, cut);
         a.splits_total = a.splits;
         if (a.splits_total > 1) reserve_records(kv, a, int64_t(kv.seqs) * count * heads);
         if (d_new_k && int64_t(count) * a.group <= kSpanRows) {
@@ -168,7 +106,7 @@ int needle2_gpu_attention_window(void *h, int layer, const float *d_q, float *d_
             st.sinks = sinks;
             launch_span_store(st, s);
         }
-        launch(a, wide, kv.head_dim, s);
+        launch(a, cut.wide, kv.head_dim, s);
         if (a.splits_total > 1) launch_span_join(a, kv.head_dim, s);
     });
 }
@@ -196,8 +134,9 @@ int needle2_gpu_attention_shared(void *h, int layer, void *prefix, int prefix_se
         SpanArgs far = span_args(kv, layer_of(pre, layer, prefix_seq), d_q, d_out, 1, heads, kv.seqs);
         far.length = prefix_length;
         const bool shared = prefix_length > 0;
-        plan(own, kv.head_dim, length, 0, 1, shared, false);
-        const bool wide = plan(far, kv.head_dim, prefix_length, prefix_length, 1, true, true);
+        use(own, cut_own(device_cus(), kv.head_dim, kv.seqs, kv.kvheads, heads, length, shared));
+        const SpanCut cut = cut_prefix(device_cus(), kv.head_dim, kv.seqs, kv.kvheads, heads, prefix_length);
+        use(far, cut);
         if (!shared) far.splits = 0;
         own.split0 = far.splits;
         own.splits_total = far.splits_total = far.splits + own.splits;
@@ -208,7 +147,7 @@ int needle2_gpu_attention_shared(void *h, int layer, void *prefix, int prefix_se
         }
         if (!shared) {
             launch_span(own, kv.head_dim, s);
-        } else if (wide) {
+        } else if (cut.wide) {
             launch_span_wide_own(far, own, kv.head_dim, s);
         } else {
             // eight waves fill a compute unit, and the launch has the sequences' own blocks too
@@ -235,7 +174,7 @@ int needle2_gpu_attention_weights(void *h, int layer, const float *d_q, float *d
         a.lengths = d_lengths;
         a.new_k = d_new_k;
         a.new_v = d_new_v;
-        plan(a, kv.head_dim, length, 0, 1, true, false);
+        use(a, cut_own(device_cus(), kv.head_dim, kv.seqs, kv.kvheads, heads, length, true));
         a.splits_total = a.splits;
         reserve_records(kv, a, int64_t(kv.seqs) * heads);  // for one piece too: the weights need the final sums
         a.score_stride = std::max(1, span_tiles(length)) * kSpanTile;

@@ -1,0 +1,301 @@
+"""The span attention's kernel for many query rows: sizes that are cut for it (tests/test_span_plan.py asserts that they
+are), against the closed form in 64 bits.
+
+Tolerance, per output: that of tests/test_span_gpu.py, and what two float16 terms leave of a value. Of a q it is at most
+2^-23 of itself, so 2^-23 of a score's terms, and further terms are taken where the rest could pass 2^-24 of a score times
+log2 e. Of p * v_scale it is at most 2^-23 of itself, so 2^-23 of sum p |V|, and 2^-26 of the largest one that the row has
+in the tile of 32 keys, among those whose V rows are not zeros (a zero row adds exactly nothing).
+"""
+import numpy as np
+import pytest
+
+from openneedle_amd.device import DeviceArray, synchronize
+from tests.test_span_gpu import EPS, Rows, check, ring_slot, run_shared, run_window, seen, upload
+
+pytestmark = pytest.mark.gpu
+
+# (sequences, kv heads, query heads per kv head, tokens, sinks, window): windows shorter and longer than the piece, one and
+# two blocks of rows, groups that do not divide a block's rows, one piece of the keys and many
+EDGES = [(16, 8, 4, 40, 3, 40), (40, 8, 3, 43, 4, 90), (20, 8, 16, 9, 0, 150), (40, 8, 3, 50, 70, 1), (16, 8, 2, 130, 0, 64),
+         (64, 8, 1, 17, 3, 40), (24, 8, 5, 64, 3, 70), (64, 8, 4, 5, 4, 60)]
+LONG = (1, 2, 2, 40, 0, 4000)     # pieces of one or two tiles
+PIECE = (32, 8, 2, 40, 0, 301)    # one piece of twelve
+# (sequences, kv heads, query heads per kv head, prefix)
+PREFIXES = [(40, 1, 4, 700), (17, 2, 3, 700), (9, 2, 4, 30011)]
+
+
+def attend(q, k, v, vs, tiles=None):
+    """(output, tolerance) of one query row over rows k, v in 64 bits; vs: the V rows' scales, tiles: the keys' tiles
+    (none: as if all were in one, which the bound of the largest weight covers)."""
+    hd = q.shape[-1]
+    if len(k) == 0:
+        return np.zeros(hd), np.zeros(hd)
+    q = q.astype(np.float64)
+    x = k @ q / np.sqrt(hd)
+    p = np.exp(x - x.max())
+    p /= p.sum()
+    size = (np.abs(k) @ np.abs(q)).max() / np.sqrt(hd)
+    score = (np.sqrt(3 * hd) + 16 + 2) * EPS * size + EPS
+    tol = (2 * score + (np.sqrt(3 * len(k)) + 8 + 2) * EPS) * (p @ np.abs(v)) + 1e-37
+    weight = np.where(v.any(-1), p * np.abs(vs), 0)
+    codes = np.abs(v) / np.where(vs == 0, 1, np.abs(vs))[:, None]
+    tiles = np.zeros(len(k), int) if tiles is None else tiles
+    for t in np.unique(tiles):
+        mine = tiles == t
+        tol = tol + 2.0 ** -26 * weight[mine].max() * codes[mine].sum(0)
+    return p @ v, tol
+
+
+def check_ring(r, q, positions, sinks, window, got, seqs, kv_heads, tokens, tiled=False):
+    """tiled: slot = position, the first row's first key at the start of a tile of 32."""
+    cap = r.k.shape[1]
+    group = q.shape[2] // r.k.shape[2]
+    for s in seqs:
+        for i in tokens:
+            at = np.array(seen(positions[s] + i, sinks, window), np.int64)
+            slots = np.where(at < sinks, at, sinks + (at - sinks) % (cap - sinks))
+            for h in kv_heads:
+                k, v = r.at(s, slots, h)
+                for g in range(h * group, h * group + group):
+                    want, tol = attend(q[s, i, g], k, v, r.vs[s, slots, h].astype(np.float64), slots // 32 if tiled else None)
+                    check(got[s, i, g], want, tol, f"sequence {s} token {i} head {g}")
+
+
+def rows_of(rng, shape, hd, extra=0, **kw):
+    seqs, kvh, group, count, sinks, window = shape
+    return Rows(rng, seqs, sinks + window + count - 1 + extra, kvh, hd, **kw)
+
+
+def queries(rng, shape, hd):
+    seqs, kvh, group, count = shape[:4]
+    return rng.normal(size=(seqs, count, kvh * group, hd)).astype(np.float32)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("shape", EDGES)
+def test_ring_edges(hd, shape):
+    """New rows stored first; left padding, before the window is full, wraps inside the piece, far positions."""
+    seqs, kvh, group, count, sinks, window = shape
+    rng = np.random.default_rng(hd + sum(shape))
+    r, q = rows_of(rng, shape, hd, extra=window % 3), queries(rng, shape, hd)
+    kinds = [0, -count, 1 - count, -2, 1, sinks + 1, window, window + sinks, 5 * window + 7, 12345, 2 ** 31 - 1 - count]
+    positions = [kinds[s % len(kinds)] for s in range(seqs)]
+    new = tuple(rng.normal(size=(seqs, count, kvh, hd)).astype(np.float32) for _ in "kv")
+    got = run_window(r, q, positions, sinks, window, new)
+    for s, first in enumerate(positions):
+        for i in range(count):
+            if first + i >= 0:
+                r.put(s, ring_slot(first + i, sinks, r.k.shape[1]), new[0][s, i], new[1][s, i])
+    r.same()
+    tokens = sorted({0, 1, 2, count // 2, count - 2, count - 1})
+    check_ring(r, q, positions, sinks, window, got, range(len(kinds)), (0, kvh - 1), tokens)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_pieces_and_rows_stored_before(hd):
+    """Many pieces of the keys; without new rows the tokens' own are taken from the cache; the second of two layers."""
+    rng = np.random.default_rng(hd)
+    r, q = rows_of(rng, LONG, hd, extra=7, layers=2, layer=1), queries(rng, LONG, hd)
+    for first in (50, 3999, 123456):
+        check_ring(r, q, [first], 0, 4000, run_window(r, q, [first], 0, 4000), [0], [0, 1], [0, 17, 39])
+
+
+def piece(rng, hd, change, q=None, tokens=range(40), kv_heads=(0, 1)):
+    """PIECE with rows as `change` leaves them, every sequence alike: token i attends positions i .. i + 300."""
+    seqs, kvh = PIECE[:2]
+    r = rows_of(rng, PIECE, hd)
+    change(r)
+    r.push()
+    q = queries(rng, PIECE, hd) if q is None else q
+    got = run_window(r, q, [300] * seqs, 0, 301)
+    check_ring(r, q, [300] * seqs, 0, 301, got, (0, seqs - 1), kv_heads, tokens, tiled=True)
+    return got
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("ratio", [1e4, 1e6, 1e8, 1e12, 1e30])
+def test_uneven_queries(hd, ratio):
+    """Entries of q far above the rest over zero K codes, in some rows only: the other entries' products decide."""
+    rng = np.random.default_rng(hd + int(np.log10(ratio)))
+    q = queries(rng, PIECE, hd)
+    q[:, 3::7, :, 5] = ratio
+    q[:, 5] *= 1e-30
+    q[:, 6] = 0
+
+    def change(r):
+        r.k[:, :, :, 5] = 0
+    piece(rng, hd, change, q, tokens=(0, 3, 5, 6, 7, 10, 39))
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("margin", [3, 10, 30, 60, 120])
+def test_dominant_slots(hd, margin):
+    """Some slots whose scores are `margin` above the rest, with zero V codes in half of the dimensions: there the other
+    slots' sums show."""
+    rng = np.random.default_rng(hd + margin)
+    sign = rng.choice([-1, 1], hd)
+    q = (np.abs(queries(rng, PIECE, hd)) * sign).astype(np.float32)
+
+    def change(r):
+        for j in (0, 77, 200):
+            r.k[:, j] = 127 * sign
+            r.ks[:, j] = margin * np.sqrt(hd) / (127 * np.abs(q).sum(-1).mean())
+            r.v[:, j, :, ::2] = 0
+    piece(rng, hd, change, q, tokens=(0, 1, 39))
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("scales", ["tiny", "huge", "zero", "signed"])
+def test_v_scales(hd, scales):
+    def change(r):
+        if scales == "tiny":
+            r.vs *= np.float32(2.0 ** -108)
+        elif scales == "huge":
+            r.vs *= np.float32(2.0 ** 118)
+        elif scales == "zero":
+            r.vs[:, :200] = 0
+        else:
+            r.vs[:, ::3] *= -1
+            r.ks[:, ::2] *= -1
+    piece(np.random.default_rng(50 + hd), hd, change, tokens=(0, 1, 20, 39))
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_non_finite_input(hd):
+    """As for few rows: a head with an infinity or NaN in its query yields zeros and leaves the others alone; an infinite
+    V scale gives infinities of the codes' signs (NaN for a zero code) to the rows that attend it, of its kv head."""
+    rng = np.random.default_rng(8 + hd)
+    seqs, kvh, group, count, sinks, window = PIECE
+    r, q = rows_of(rng, PIECE, hd), queries(rng, PIECE, hd)
+    q[0, 0, 0, 3] = np.nan
+    q[0, 1, 1, 9] = np.inf
+    q[0, 39, 2, hd - 1] = -np.inf
+    first = [300] * seqs
+    got = run_window(r, q, first, 0, 301)
+    for i, h in ((0, 0), (1, 1), (39, 2)):
+        assert not got[0, i, h].any()
+        q[0, i, h] = 0  # and what any finite query gives, for the check below
+    again = run_window(r, q, first, 0, 301)
+    for i, h in ((0, 0), (1, 1), (39, 2)):
+        got[0, i, h] = again[0, i, h]
+    np.testing.assert_array_equal(got, again)
+    check_ring(r, q, first, 0, 301, got, [0, 1], [0, 1], [0, 1, 2, 39])
+    r.vs[0, 20, 1] = np.inf  # attended by tokens 0 to 20 only
+    r.v[0, 20, 1, 3] = 0
+    r.push()
+    got = run_window(r, q, first, 0, 301)
+    codes = r.v[0, 20, 1]
+    want = np.where(codes == 0, np.nan, np.where(codes > 0, np.inf, -np.inf))
+    for i in (0, 20):
+        for h in (2, 3):
+            np.testing.assert_array_equal(got[0, i, h], want)
+    check_ring(r, q, first, 0, 301, got, [0], [1], [21, 39])
+    check_ring(r, q, first, 0, 301, got, [0, 1], [0], [0, 20, 39])
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("value", [np.nan, np.inf, 3e38, 1e-38])
+def test_what_is_not_attended_does_not_matter(hd, value):
+    """Slots outside the window hold scales that are infinite, NaN or at the ends of the range."""
+    rng = np.random.default_rng(6)
+    seqs, kvh, group, count, sinks, window = shape = EDGES[0]
+    r, q = rows_of(rng, shape, hd, extra=90), queries(rng, shape, hd)
+    cap = r.k.shape[1]
+    positions = [(0, 20, 300, 501)[s % 4] for s in range(seqs)]
+    for s, first in enumerate(positions):
+        live = {ring_slot(j, sinks, cap) for i in range(count) for j in seen(first + i, sinks, window)}
+        dead = [j for j in range(cap) if j not in live]
+        assert dead
+        r.ks[s, dead] = value
+        r.vs[s, dead] = value
+    r.push()
+    got = run_window(r, q, positions, sinks, window)
+    check_ring(r, q, positions, sinks, window, got, range(4), (0, 7), (0, 1, 20, 38, 39))
+
+
+def test_unaligned_buffers():
+    """q and the output start at any float."""
+    rng = np.random.default_rng(33)
+    seqs, kvh, group, count, sinks, window = shape = EDGES[1]
+    r, q = rows_of(rng, shape, 64), queries(rng, shape, 64)
+    d_n, big = upload([299] * seqs, np.int32), [DeviceArray(q.nbytes + 16) for _ in range(2)]
+    for off in (4, 8, 12):
+        d_q, d_o = (b.view(off, q.nbytes) for b in big)
+        d_q.upload(q)
+        r.kv.attention_window(0, d_q, d_o, kvh * group, count, d_n, sinks, window)
+        synchronize()
+        check_ring(r, q, [299] * seqs, sinks, window, d_o.to_host(np.float32, q.shape), [0], [0, kvh - 1], (0, 17, count - 1))
+
+
+def test_same_results_every_time():
+    rng = np.random.default_rng(30)
+    for shape, first in ((PIECE, 300), (LONG, 5000)):
+        r, q = rows_of(rng, shape, 128), queries(rng, shape, 128)
+        one = run_window(r, q, [first] * shape[0], 0, shape[5])
+        for _ in range(3):
+            np.testing.assert_array_equal(run_window(r, q, [first] * shape[0], 0, shape[5]), one)
+
+
+# ---- a shared prefix --------------------------------------------------------------------------------------------------
+def shared(rng, shape, hd, change=None, q=None, seqs=(0, 1, -1), tiled=True):
+    n, kvh, group, length = shape
+    prefix, r = Rows(rng, 1, length + 3, kvh, hd), Rows(rng, n, 70, kvh, hd)
+    if change:
+        change(prefix, r)
+        prefix.push()
+        r.push()
+    q = rng.normal(size=(n, kvh * group, hd)).astype(np.float32) if q is None else q
+    lengths = rng.integers(1, 70, n)
+    lengths[1] = 0
+    got = run_shared(r, prefix, length, q, 70, lengths)
+    for h in range(kvh):
+        pk, pv = prefix.at(0, range(length), h)
+        for s in seqs:
+            k, v = r.at(s, range(lengths[s]), h)
+            both = np.concatenate([pk, k]), np.concatenate([pv, v])
+            vs = np.concatenate([prefix.vs[0, :length, h], r.vs[s, :lengths[s], h]]).astype(np.float64)
+            # (the sequences' own slots have exact weights: any tiles cover them)
+            tiles = np.concatenate([np.arange(length) // 32, 10 ** 6 + np.arange(lengths[s])])
+            for g in range(h * group, h * group + group):
+                want, tol = attend(q[s, g], *both, vs, tiles if tiled else None)
+                check(got[s, g], want, tol, f"sequence {s} head {g}")
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("shape", PREFIXES)
+def test_prefix(hd, shape):
+    shared(np.random.default_rng(hd + shape[0]), shape, hd)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("scales", ["tiny", "huge", "zero", "signed", "infinite"])
+def test_prefix_v_scales(hd, scales):
+    def change(p, r):
+        if scales == "tiny":
+            p.vs *= np.float32(2.0 ** -108)
+            r.vs *= np.float32(2.0 ** -108)
+        elif scales == "huge":
+            p.vs *= np.float32(2.0 ** 118)
+        elif scales == "zero":
+            p.vs[:, :20000] = 0
+        elif scales == "signed":
+            p.vs[:, ::3] *= -1
+            p.ks[:, ::2] *= -1
+        else:  # behind the prefix
+            p.vs[:, -3:] = np.inf
+            p.ks[:, -2:] = np.nan
+    shared(np.random.default_rng(60 + hd), PREFIXES[2], hd, change)
+
+
+def test_prefix_non_finite_query():
+    rng = np.random.default_rng(70)
+    n, kvh, group, length = PREFIXES[0]
+    prefix, r = Rows(rng, 1, length, kvh, 64), Rows(rng, n, 8, kvh, 64)
+    q = rng.normal(size=(n, kvh * group, 64)).astype(np.float32)
+    clean = run_shared(r, prefix, length, q, 8, None)
+    q[3, 1, 7] = np.nan
+    q[39, 3, 0] = -np.inf
+    got = run_shared(r, prefix, length, q, 8, None)
+    assert not got[3, 1].any() and not got[39, 3].any()
+    clean[3, 1] = clean[39, 3] = 0
+    np.testing.assert_array_equal(got, clean)

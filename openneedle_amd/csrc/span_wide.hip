@@ -2,11 +2,16 @@
 // prefix. The mathematics and the records are span_kernels.hip's. The matrix instructions bound this kernel, so both
 // products run on v_mfma_f32_32x32x16_f16 with q and p * vs as two float16 terms (the codes are float16 numbers as they
 // are) instead of three bfloat16 ones: 22 bits of a value, and of small values what lies above 2^-25 of the term's unit.
-//   q is scaled by a power of two so that the row's largest |q| is in [2^14, 2^15). What the terms leave is below 2^-25
-//   there, 2^-25 * 127 HD * |ks| in a score; where that could pass 2^-24 (of a score times log2 e, whose own rounding is
-//   2^-24 of its size) the tile's scores get the rest of q in further terms, until nothing is left.
-//   p * vs is scaled so that the largest of a row's 32 in a tile is at least 2^2: what the terms leave is below 2^-27 of
-//   it, where an fp32 sum of the 32 rounds by 2^-24 of its largest term.
+//   q is scaled by a power of two so that the row's largest |q| is in [2^14, 2^15). Of a value the terms leave at most
+//   2^-23 (the last bit of a quarter of them; the sums round by as much), of a small one at most 2^-25, together
+//   2^-25 * 127 HD * |ks| in a score; where that could pass 2^-24 (of a score times log2 e, whose own rounding is 2^-24 of its
+//   size) the tile's scores get the rest of q in further terms, until nothing is left.
+//   p * vs is scaled by one power of two a row, 2^(kLift - M), that follows the largest score and the largest V scale, and of
+//   it the terms leave at most 2^-23, of a small one 2^-25: 2^-26 of the row's largest in the tile, where that is at least 2
+//   (an fp32 sum of the 32 rounds by 2^-24 of its largest term). Where it is not (the largest V scale is another key's, or
+//   one's that the row does not attend; or the scores are far below the row's largest), the tile is added with a power of
+//   two of its own a row, whose largest is then in [2^9, 2^10). Held in fp32 before that, a weight below 2^-119 of the row's
+//   largest V scale may be lost.
 // 6 x 999 tokens, 32 heads of 128 values, window 2048: 428 us, 1.0 PFLOP/s of matrix work (a large bfloat16 product of the
 // library reaches 1.2). The matrix unit is busy 47% of the cycles; the rest is the softmax and the making of terms, 258
 // vector instructions a wave and tile next to its 32 matrix instructions. Rows of 64: 362 us. A third block a
@@ -96,12 +101,9 @@ __device__ __forceinline__ u32x4 widen_half(uint32_t a, uint32_t b) {
 
 // The row's outputs and sum are held times 2^(kLift - M): M is a whole number, at least the largest score (times log2 e)
 // plus the exponent of its tile's largest V scale, less kSlack (so it moves, and the outputs are rescaled, in few tiles).
-// For a tile that lies kDrop or more below M for some row the outputs are scaled up to that tile's own largest weights and
-// back, by powers of two: exactly.
-constexpr float kLift = 10.0f, kSlack = 5.0f, kDrop = 8.0f;
+constexpr float kLift = 10.0f, kSlack = 5.0f;
 constexpr int kMostExp = 50;  // of a V scale that M follows: the sum, which M scales too, stays far from underflow
 constexpr int kOddTile = 1024;
-constexpr int kMostUp = 80;   // of a scaling to a tile's own weights: the outputs stay far from overflow
 
 constexpr int kFrag = 66;  // 16-byte lanes of an operand in LDS: 32, one of padding (the halves in different banks), 32, 1
 __device__ __forceinline__ int frag_lane(int m, int half) { return m + 33 * half; }
@@ -346,6 +348,36 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
         }
     };
 
+    // A tile whose weights w are too small for float16, too large, or not finite: its terms are of w times the row's own
+    // power of two 2^-unit, and so are the outputs while it is added (as far as they stay below 2^100).
+    auto rescale = [&](Halves (&p)[2], const f32x16 &w, uint32_t gone) {
+        float y[16], most = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            y[j] = gone >> j & 1u ? 0.0f : w[j];  // (0 times a scale that is no number)
+            most = fmaxf(most, fabsf(y[j]) < INFINITY ? fabsf(y[j]) : 0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sum = fmaxf(sum, fabsf(acc[i][j]) < INFINITY ? fabsf(acc[i][j]) : 0.0f);
+        most = fmaxf(most, butterfly_partner<32>(most, lane));
+        sum = fmaxf(sum, butterfly_partner<32>(sum, lane));
+        int unit = most > 0 ? max(-126, __builtin_amdgcn_frexp_expf(most) - 10) : 0;
+        if (sum > 0) unit = max(unit, __builtin_amdgcn_frexp_expf(sum) - 100);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            float z[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] = ldexpf(y[8 * ks + j], -unit);
+            p[ks] = halve8_any(z);
+        }
+        const float to = ldexpf(1.0f, -unit);
+#pragma unroll
+        for (int i = 0; i < DT; ++i) acc[i] *= to;
+        return unit;
+    };
+
     place_k(rk_first, begin);
     place_k(rk_next, begin + 1);
     place_v(rv_next, begin);
@@ -359,8 +391,7 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
         const int vb = (tile - begin) & 1, sb = (tile - begin) & 3;
         const int s0 = slot0(tile), behind = stop(tile);
         const int code = __builtin_amdgcn_readfirstlane(about[sb].x);
-        const bool odd = code > kOddTile / 2;
-        const int ve = odd ? code - kOddTile : code;
+        const int ve = code > kOddTile / 2 ? code - kOddTile : code;
         f32x16 x;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -378,6 +409,7 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
                                  : s0 < runs.pinned || s0 + shift <= full_low || s0 + kWideTile - 1 + shift > full_high;
         }
         uint32_t gone = 0;  // this lane's keys that the row does not attend
+        uint32_t idle = 0;  // rows that attend none of the tile's
         if (masked) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -391,29 +423,24 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
                 x[j] = ok ? x[j] : -INFINITY;
                 gone |= ok ? 0u : 1u << j;
             }
+            const uint64_t none = __ballot(gone == 0xFFFFu);
+            idle = static_cast<uint32_t>(none) & static_cast<uint32_t>(none >> 32);
         }
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 16; ++j) top = fmaxf(top, x[j]);
         top = fmaxf(top, butterfly_partner<32>(top, lane)) * down;
         const int follow = max(-kMostExp, min(kMostExp, ve));
-        const float high = ceilf(top) + static_cast<float>(follow);
-        const int beyond = ve - follow;
-        bool apart = false;
-        float up = 0.0f;
-        // (high above M = -inf: the first scores)
-        if (beyond != 0 || __any(high > M + kSlack || (high < M - kDrop && high > -INFINITY))) {
+        const float high = ceilf(top) + static_cast<float>(max(-kMostExp, min(kMostExp, ve)));
+        if (__any(high > M + kSlack)) {  // (above M = -inf: the first scores)
             const float most = fmaxf(M, high);
             const float alpha = M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - most);
             M = most;
-            apart = beyond != 0 || __any(high < M - kDrop && high > -INFINITY);
-            if (apart && high > -INFINITY) up = fminf(M - high, static_cast<float>(min(kMostUp, kMostUp + beyond)));
-            l *= alpha * __builtin_amdgcn_exp2f(up);
-            const float grow = alpha * __builtin_amdgcn_exp2f(up - static_cast<float>(beyond));
+            l *= alpha;
 #pragma unroll
-            for (int i = 0; i < DT; ++i) acc[i] *= grow;
+            for (int i = 0; i < DT; ++i) acc[i] *= alpha;
         }
-        const float lifted = M > -INFINITY ? kLift + up - M : 0.0f;  // nothing attended yet: every power is 0
+        const float lifted = M > -INFINITY ? kLift - M : 0.0f;  // nothing attended yet: every power is 0
         // the next tile's product beside this tile's weights (ahead of the other block's wave: 466 -> 456 us where the
         // matrix unit is the bound)
         __builtin_amdgcn_s_setprio(1);
@@ -438,16 +465,13 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
             for (int j = 0; j < 8; ++j) w[j] = x[8 * ks + j];
             p[ks] = halve8(w);
         }
-        if (odd || beyond != 0) {  // scales that are no numbers or far from 1: masked weights may be NaN, others infinite
-            const float shrink = __builtin_amdgcn_exp2f(static_cast<float>(-beyond));
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                float w[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = gone >> (8 * ks + j) & 1u ? 0.0f : x[8 * ks + j] * shrink;
-                p[ks] = halve8_any(w);
-            }
-        }
+        // a row none of whose weights reaches 2 (the first bit of a float16 exponent), though it attends some of the keys
+        const uint32_t bits = (p[0].hi.x | p[0].hi.y | p[0].hi.z | p[0].hi.w) | (p[1].hi.x | p[1].hi.y | p[1].hi.z | p[1].hi.w);
+        const uint64_t held = __ballot((bits & 0x40004000u) != 0);
+        const bool apart =
+            code > kMostExp || (static_cast<uint32_t>(held) | static_cast<uint32_t>(held >> 32) | idle) != ~0u;
+        int unit = 0;
+        if (apart) unit = rescale(p, x, gone);
         // this tile's values beside the operands of the tiles to come
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -460,10 +484,9 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
         place_k(rk_next, tile + 2);
         __builtin_amdgcn_s_setprio(0);
         if (apart) {
-            l *= __builtin_amdgcn_exp2f(-up);
-            const float back = __builtin_amdgcn_exp2f(static_cast<float>(beyond) - up);
+            const float from = ldexpf(1.0f, unit);
 #pragma unroll
-            for (int i = 0; i < DT; ++i) acc[i] *= back;
+            for (int i = 0; i < DT; ++i) acc[i] *= from;
         }
         finish_product(next, tile + 1);
         fetch_k(rk_next, tile + 3);

@@ -145,13 +145,17 @@ def test_dominant_slots(hd, margin):
 
 
 @pytest.mark.parametrize("hd", [32, 64, 128])
-@pytest.mark.parametrize("scales", ["tiny", "huge", "zero", "signed"])
+@pytest.mark.parametrize("scales", ["tiny", "huge", "mixed", "zero", "signed"])
 def test_v_scales(hd, scales):
     def change(r):
         if scales == "tiny":
             r.vs *= np.float32(2.0 ** -108)
         elif scales == "huge":
             r.vs *= np.float32(2.0 ** 118)
+        elif scales == "mixed":
+            r.vs[:, :160] *= np.float32(2.0 ** -100)
+            r.vs[:, 100] = 2.0 ** 90
+            r.vs[:, 200:] *= np.float32(2.0 ** -30)
         elif scales == "zero":
             r.vs[:, :200] = 0
         else:
@@ -268,7 +272,7 @@ def test_prefix(hd, shape):
 
 
 @pytest.mark.parametrize("hd", [32, 64, 128])
-@pytest.mark.parametrize("scales", ["tiny", "huge", "zero", "signed", "infinite"])
+@pytest.mark.parametrize("scales", ["tiny", "huge", "mixed", "zero", "signed", "infinite"])
 def test_prefix_v_scales(hd, scales):
     def change(p, r):
         if scales == "tiny":
@@ -276,6 +280,10 @@ def test_prefix_v_scales(hd, scales):
             r.vs *= np.float32(2.0 ** -108)
         elif scales == "huge":
             p.vs *= np.float32(2.0 ** 118)
+        elif scales == "mixed":
+            p.vs[:, :16000] *= np.float32(2.0 ** -100)
+            p.vs[:, 10000] = 2.0 ** 90
+            r.vs *= np.float32(2.0 ** -30)
         elif scales == "zero":
             p.vs[:, :20000] = 0
         elif scales == "signed":
@@ -299,3 +307,61 @@ def test_prefix_non_finite_query():
     assert not got[3, 1].any() and not got[39, 3].any()
     clean[3, 1] = clean[39, 3] = 0
     np.testing.assert_array_equal(got, clean)
+
+
+# ---- V scales of a tile far apart ---------------------------------------------------------------------------------------
+def dominant(q, rows, at, margin):
+    """Slot `at` of every sequence with scores about `margin` above the rest; q gets one sign a dimension."""
+    hd = q.shape[-1]
+    sign = np.where(np.arange(hd) % 3 == 0, -1, 1)
+    q[:] = np.abs(q) * sign
+    rows.k[:, at] = 127 * sign
+    rows.ks[:, at] = margin * np.sqrt(hd) / (127 * np.abs(q).sum(-1).mean())
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("apart", [8, 12, 16, 20, 24, 30, 36, 60])
+def test_the_largest_score_at_a_small_v_scale(hd, apart):
+    rng = np.random.default_rng(apart)
+    q = queries(rng, PIECE, hd)
+
+    def change(r):
+        dominant(q, r, 77, 30)
+        r.vs[:, 77] *= np.float32(2.0 ** -apart)
+    piece(rng, hd, change, q, tokens=(0, 1, 39))
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("apart", [8, 15, 20, 25, 30, 40, 60, 100, 120])
+def test_v_scales_of_keys_that_a_row_does_not_attend(hd, apart):
+    """Position 310 is attended by the tokens from 10 on, position 5 by those up to 5; their tiles by all. Both V scales are
+    2^apart times the rest's."""
+    def change(r):
+        r.vs[:, 310] = r.vs[:, 5] = np.float32(0.015 * 2.0 ** apart)
+    piece(np.random.default_rng(apart), hd, change, tokens=(0, 5, 6, 9, 10, 39))
+
+
+@pytest.mark.parametrize("hd", [32, 128])
+def test_v_scales_that_change_from_tile_to_tile(hd):
+    """The outputs meet weights far larger and far smaller than themselves, in every order."""
+    rng = np.random.default_rng(hd)
+
+    def change(r):
+        for t, e in enumerate((0, 60, -60, 30, -100, 90, -20, 110, -110, 10, -50)):
+            r.vs[:, 32 * t:32 * t + 32] *= np.float32(2.0 ** e)
+            r.v[:, 32 * t:32 * t + 32, :, t:t + 1] = 0  # where the tile's own codes are zeros the others show
+    piece(rng, hd, change, tokens=(0, 39))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("apart", [12, 24, 36])
+def test_prefix_the_largest_score_at_a_small_v_scale(hd, apart):
+    rng = np.random.default_rng(apart + 1)
+    n, kvh, group, length = PREFIXES[2]
+    q = rng.normal(size=(n, kvh * group, hd)).astype(np.float32)
+
+    def change(p, r):
+        dominant(q, p, 7777, 30)
+        p.vs[:, 7777] *= np.float32(2.0 ** -apart)
+        r.vs *= np.float32(2.0 ** -apart)
+    shared(rng, PREFIXES[2], hd, change, q)

@@ -10,8 +10,8 @@
 //   it the terms leave at most 2^-23, of a small one 2^-25: 2^-26 of the row's largest in the tile, where that is at least 2
 //   (an fp32 sum of the 32 rounds by 2^-24 of its largest term). Where it is not (the largest V scale is another key's, or
 //   one's that the row does not attend; or the scores are far below the row's largest), the tile is added with a power of
-//   two of its own a row, whose largest is then in [2^9, 2^10). Held in fp32 before that, a weight below 2^-119 of the row's
-//   largest V scale may be lost.
+//   two of its own a row, whose largest is then in [2^9, 2^10). V rows of zeros as the cache stores them (scale 1) count
+//   for none of this. Held in fp32 before that, a weight below 2^-119 of the row's largest V scale may be lost.
 // 6 x 999 tokens, 32 heads of 128 values, window 2048: 428 us, 1.0 PFLOP/s of matrix work (a large bfloat16 product of the
 // library reaches 1.2). The matrix unit is busy 47% of the cycles; the rest is the softmax and the making of terms, 258
 // vector instructions a wave and tile next to its 32 matrix instructions. Rows of 64: 362 us. A third block a
@@ -208,7 +208,17 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
         }
         if (wave == kScaleWave) {
             const bool in = slot0(tile) + col < stop(tile);
-            const float ks = in ? r.s[0] * a.scale : 0.0f, vs = in ? r.s[1] : 0.0f;
+            const float ks = in ? r.s[0] * a.scale : 0.0f;
+            float vs = in ? r.s[1] : 0.0f;
+            // A V row of zeros, whose scale the quantiser makes 1, adds nothing: scale 0, so that neither M nor a row's
+            // largest weight is taken from it.
+            if (__any(vs == 1.0f)) {
+                u32x4 codes = {0, 0, 0, 0};
+#pragma unroll 1
+                for (int c = 0; c < HD && __any(vs == 1.0f && (codes.x | codes.y | codes.z | codes.w) == 0); c += 16)
+                    codes |= __builtin_amdgcn_raw_buffer_load_b128(rv, (static_cast<uint32_t>(slot0(tile)) + col) * HD + c, 0, 0);
+                if (vs == 1.0f && (codes.x | codes.y | codes.z | codes.w) == 0) vs = 0.0f;
+            }
             sc[sb][half][col] = half ? vs : ks;
             const float v = fabsf(vs);
             const bool odd = !(v < INFINITY);

@@ -365,3 +365,56 @@ def test_prefix_the_largest_score_at_a_small_v_scale(hd, apart):
         p.vs[:, 7777] *= np.float32(2.0 ** -apart)
         r.vs *= np.float32(2.0 ** -apart)
     shared(rng, PREFIXES[2], hd, change, q)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("apart", [0, 8, 16, 20, 24, 30, 36, 60])
+@pytest.mark.parametrize("margin", [0, 30])
+def test_v_rows_of_zeros(hd, apart, margin):
+    """A V row of zeros as the cache stores it (scale 1), the others' scales 2^apart below; its score is like the others'
+    or far ahead of them. Two such rows in a tile, and a row of which only one value is not zero."""
+    rng = np.random.default_rng(apart + margin)
+    q = queries(rng, PIECE, hd)
+
+    def change(r):
+        r.vs *= np.float32(2.0 ** -apart)
+        for at in (77, 79, 160, 319):
+            if margin and at != 160:
+                dominant(q, r, at, margin)
+            r.v[:, at] = 0
+            r.vs[:, at] = 1
+        r.v[:, 78] = 0
+        r.v[:, 78, :, hd - 1] = 3
+        r.vs[0, 200, 1] = np.nan if apart == 36 else r.vs[0, 200, 1]
+        r.v[0, 200, 1] = 0 if apart == 36 else r.v[0, 200, 1]
+    got = piece(rng, hd, change, q, tokens=(0, 1, 39), kv_heads=(0,) if apart == 36 else (0, 1))
+    if apart == 36:  # zeros with a scale that is no number
+        assert np.isnan(got[0, :, 2:4]).all()
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_prefix_v_rows_of_zeros(hd):
+    rng = np.random.default_rng(hd)
+    n, kvh, group, length = PREFIXES[2]
+    q = rng.normal(size=(n, kvh * group, hd)).astype(np.float32)
+
+    def change(p, r):
+        dominant(q, p, 7777, 60)
+        p.v[:, [7777, 64, 0, 30010]] = 0
+        p.vs *= np.float32(2.0 ** -20)
+        r.vs *= np.float32(2.0 ** -20)
+        p.vs[:, [7777, 64, 0, 30010]] = 1
+    shared(rng, PREFIXES[2], hd, change, q)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_v_scales_of_one(hd):
+    """Rows of the scale that rows of zeros have, zeros in all but their last codes."""
+    rng = np.random.default_rng(hd)
+
+    def change(r):
+        r.vs[:] = 1
+        r.v[:, ::5, :, :hd - 1] = 0
+        r.v[:, ::5, :, hd - 1] = 1
+        r.v[:, ::15] = 0
+    piece(rng, hd, change, tokens=(0, 39))

@@ -63,10 +63,12 @@ def test_the_many_row_kernels_tests_reach_it(host, hd):
     assert window(host, hd, wide.LONG, 7)["wide"] and window(host, hd, wide.LONG)["splits"] > 8
     one = window(host, hd, wide.PIECE)
     assert one["wide"] and one["splits"] == 1
-    for n, kvh, group, length in wide.PREFIXES:
+    for n, kvh, group, length in [*wide.PREFIXES, wide.GRAPH_PREFIX]:
         assert call(host.prefix_cut, hd, n, kvh, kvh * group, length)["wide"], (n, kvh, group, length)
     n, kvh, group, length = wide.PREFIXES[2]
     assert call(host.prefix_cut, hd, n, kvh, kvh * group, length)["per"] > 1
+    one, more = ((window(host, 64, s)["splits"] * s[1] * s[2] * s[3]) for s in (wide.GRAPH_WINDOW, wide.GRAPH_OUTGROWN))
+    assert more > one  # records
 
 
 @pytest.mark.parametrize("hd", [32, 64, 128])

@@ -9,7 +9,8 @@ in the tile of 32 keys, among those whose V rows are not zeros (a zero row adds 
 import numpy as np
 import pytest
 
-from openneedle_amd.device import DeviceArray, synchronize
+from openneedle_amd.device import DeviceArray, Graph, Stream, synchronize
+from tests.test_evict_gpu import read_rows
 from tests.test_span_gpu import EPS, Rows, check, ring_slot, run_shared, run_window, seen, upload
 
 pytestmark = pytest.mark.gpu
@@ -22,6 +23,7 @@ LONG = (1, 2, 2, 40, 0, 4000)     # pieces of one or two tiles
 PIECE = (32, 8, 2, 40, 0, 301)    # one piece of twelve
 # (sequences, kv heads, query heads per kv head, prefix)
 PREFIXES = [(40, 1, 4, 700), (17, 2, 3, 700), (9, 2, 4, 30011)]
+GRAPH_WINDOW, GRAPH_PREFIX, GRAPH_OUTGROWN = LONG, (40, 2, 2, 700), (1, 2, 8, 300, 0, 3740)
 
 
 def attend(q, k, v, vs, tiles=None):
@@ -418,3 +420,78 @@ def test_v_scales_of_one(hd):
         r.v[:, ::5, :, hd - 1] = 1
         r.v[:, ::15] = 0
     piece(rng, hd, change, tokens=(0, 39))
+
+
+# ---- captured -----------------------------------------------------------------------------------------------------------
+def test_graph_replays_match_eager():
+    """A window step and a shared-prefix step of the many-row kernel, a recorded step and a cut in place whose list is the
+    handle's scratch, captured into one graph and replayed with other inputs. Between the replays eager calls of larger
+    sizes on the same handles outgrow the scratch of each."""
+    hd, cap, keep = 64, 300, 100
+    _, kvh, group, count, sinks, window = GRAPH_WINDOW
+    n, _, _, prefix = GRAPH_PREFIX
+    heads = kvh * group
+
+    def state():
+        rng = np.random.default_rng(1)
+        d = dict(ring=rows_of(rng, GRAPH_WINDOW, hd), own=Rows(rng, n, cap, kvh, hd), prefix=Rows(rng, 1, prefix, kvh, hd))
+        for name, size in dict(q=count * heads, nk=count * kvh, nv=count * kvh, o=count * heads, q1=n * heads, k1=n * kvh,
+                               v1=n * kvh, o1=n * heads, o2=n * heads).items():
+            d[name] = DeviceArray(size * hd * 4)
+        d["pos"], d["n"], d["w"] = DeviceArray(4), DeviceArray(n * 4), DeviceArray(n * kvh * cap * 4)
+        d["big_q"], d["big_o"] = (DeviceArray(GRAPH_OUTGROWN[3] * 8 * heads * hd * 4) for _ in "qo")
+        d["big_w"] = DeviceArray(n * kvh * cap * 4)
+        return d
+
+    def feed(d, seed):
+        rng = np.random.default_rng(seed)
+        for name in ("q", "nk", "nv", "q1", "k1", "v1"):
+            d[name].upload(rng.normal(size=d[name].nbytes // 4).astype(np.float32))
+        d["pos"].upload(rng.integers(0, 9000, 1).astype(np.int32))
+        d["n"].upload(rng.integers(50, cap, n).astype(np.int32))
+        d["w"].upload(rng.random(n * kvh * cap).astype(np.float32))
+
+    def step(d, stream):
+        d["ring"].kv.attention_window(0, d["q"], d["o"], heads, count, d["pos"], sinks, window, stream=stream,
+                                      new=(d["nk"], d["nv"]))
+        d["own"].kv.attention_shared(0, d["prefix"].kv, prefix, d["q1"], d["o1"], heads, cap, d["n"], stream=stream,
+                                     new=(d["k1"], d["v1"]))
+        d["own"].kv.attention_weights(0, d["q1"], d["o2"], d["w"], heads, cap, d["n"], stream=stream)
+        d["own"].kv.evict(0, d["w"], d["n"], keep, 4, 32, d["w"], d["n"], stream=stream)
+
+    def outgrow(d, stream, i):
+        """More query rows and heads, so more records and scores; a larger keep."""
+        more = heads * (2, 4, 8, 8)[i]
+        d["big_q"].fill(0)
+        d["big_w"].fill(0)
+        _, _, many, tokens, _, span = GRAPH_OUTGROWN
+        d["ring"].kv.attention_window(0, d["big_q"], d["big_o"], kvh * many, tokens, d["pos"], 0, span, stream=stream)
+        d["own"].kv.attention_shared(0, d["prefix"].kv, prefix, d["big_q"], d["big_o"], more, cap, stream=stream)
+        d["own"].kv.attention_weights(0, d["big_q"], d["big_o"], d["big_w"], more, cap, stream=stream)
+        d["own"].kv.evict(0, d["big_w"], d["n"], keep + 50 * (i + 1), 4, 32, d["big_w"], d["n"], stream=stream)
+        stream.synchronize()
+
+    def results(d):
+        return [d[k].to_host(np.uint32, d[k].nbytes // 4) for k in ("o", "o1", "o2", "w", "n")] + \
+            [a for name in ("ring", "own") for a in read_rows(d[name].kv, 0)]
+
+    stream = Stream()
+    graphed, eager = state(), state()
+    for d in (graphed, eager):
+        feed(d, 2)
+        step(d, stream)
+        stream.synchronize()
+    with Graph.capture(stream) as g:
+        step(graphed, stream)
+    for i in range(4):
+        for d in (graphed, eager):
+            feed(d, 10 + i)
+        g.launch(stream)
+        stream.synchronize()
+        step(eager, stream)
+        stream.synchronize()
+        for a, b in zip(results(graphed), results(eager)):
+            np.testing.assert_array_equal(a, b)
+        for d in (graphed, eager):
+            outgrow(d, stream, i)
+    g.close()

@@ -347,6 +347,9 @@ int needle2_gpu_attention_weights(void *kv, int layer, const float *d_q, float *
  * d_new_weights (may be d_weights, else disjoint) gets the kept weights and
  * zeros up to the capacity, d_new_lengths[s] (may be d_lengths) min(n, keep),
  * d_kept ([seqs][kvheads][keep], nullable) the old slots, -1 past the last.
+ * A call cuts one layer, and every layer's needs the lengths from before the
+ * cut: with several layers sharing d_lengths, d_new_lengths is another array
+ * (or d_lengths for the last layer only).
  * sinks + recent <= keep <= capacity, keep >= 1. */
 int needle2_gpu_kv_evict(void *kv, int layer, const float *d_weights, const int *d_lengths, int keep, int sinks,
                          int recent, float *d_new_weights, int *d_new_lengths, int *d_kept, void *stream);

@@ -107,7 +107,8 @@ class KVCache:
         ``recent`` and, of those between, the ones with the largest ``d_weights`` (of equal ones the lower slots) move to
         slots ``0 .. keep - 1`` in their order. ``d_new_weights`` (may be ``d_weights``): the kept slots' weights, then
         zeros; ``d_new_lengths`` (may be ``d_lengths``): the slots left; ``d_kept``: int32 ``[seqs][kvheads][keep]``, the
-        old slots (-1 past the last). Capturable."""
+        old slots (-1 past the last). Every layer's call needs the lengths from before the cut: where layers share
+        ``d_lengths``, only the last one's may overwrite it. Capturable."""
         check(self._lib.needle2_gpu_kv_evict(self.ptr, layer, addr(d_weights), addr(d_lengths), int(keep), int(sinks),
                                              int(recent), addr(d_new_weights), addr(d_new_lengths), addr(d_kept),
                                              stream_ptr(stream)), "eviction")

@@ -101,8 +101,12 @@ __device__ __forceinline__ u32x4 widen_half(uint32_t a, uint32_t b) {
 
 // The row's outputs and sum are held times 2^(kLift - M): M is a whole number, at least the largest score (times log2 e)
 // plus the exponent of its tile's largest V scale, less kSlack (so it moves, and the outputs are rescaled, in few tiles).
-constexpr float kLift = 10.0f, kSlack = 5.0f;
+// While a tile is added that lies kDrop or more below M, or whose weights are small for another reason, its weights and the
+// outputs are held times another power of two, at most 2^kMostUp: the outputs, below 2^48 (2^21 tiles of 32 weights below
+// 2^15 times 127), stay finite.
+constexpr float kLift = 10.0f, kSlack = 5.0f, kDrop = 7.0f;
 constexpr int kMostExp = 50;  // of a V scale that M follows: the sum, which M scales too, stays far from underflow
+constexpr int kMostUp = 76;
 constexpr int kOddTile = 1024;
 
 constexpr int kFrag = 66;  // 16-byte lanes of an operand in LDS: 32, one of padding (the halves in different banks), 32, 1
@@ -212,12 +216,14 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
             float vs = in ? r.s[1] : 0.0f;
             // A V row of zeros, whose scale the quantiser makes 1, adds nothing: scale 0, so that neither M nor a row's
             // largest weight is taken from it.
-            if (__any(vs == 1.0f)) {
-                u32x4 codes = {0, 0, 0, 0};
-#pragma unroll 1
-                for (int c = 0; c < HD && __any(vs == 1.0f && (codes.x | codes.y | codes.z | codes.w) == 0); c += 16)
-                    codes |= __builtin_amdgcn_raw_buffer_load_b128(rv, (static_cast<uint32_t>(slot0(tile)) + col) * HD + c, 0, 0);
-                if (vs == 1.0f && (codes.x | codes.y | codes.z | codes.w) == 0) vs = 0.0f;
+            if (__builtin_expect(__any(vs == 1.0f), 0)) {
+                uint32_t codes = 0;  // of a half of the row
+#pragma unroll
+                for (int c = 0; c < HD / 2; c += 4)
+                    codes |= __builtin_amdgcn_raw_buffer_load_b32(
+                        rv, (static_cast<uint32_t>(slot0(tile)) + col) * HD + half * (HD / 2) + c, 0, 0);
+                const float mine = codes != 0 ? 1.0f : 0.0f, other = butterfly_partner<32>(mine, lane);
+                if (vs == 1.0f && mine + other == 0.0f) vs = 0.0f;
             }
             sc[sb][half][col] = half ? vs : ks;
             const float v = fabsf(vs);
@@ -358,31 +364,36 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
         }
     };
 
-    // A tile whose weights w are too small for float16, too large, or not finite: its terms are of w times the row's own
-    // power of two 2^-unit, and so are the outputs while it is added (as far as they stay below 2^100).
-    auto rescale = [&](Halves (&p)[2], const f32x16 &w, uint32_t gone) {
-        float y[16], most = 0.0f, sum = 0.0f;
+    // A tile of weights w too small for float16, too large, or not finite: w, and the outputs while it is added, are held
+    // times the row's own power of two 2^-unit (next to the 2^up that they are held times already).
+    bool wide_range = false;  // a V scale above 2^kMostExp has been met: the outputs' size has to be looked at
+    auto rescale = [&](f32x16 &w, uint32_t gone, bool far, float up) {
+        wide_range = wide_range || far;
+        float most = 0.0f;
+        int least = static_cast<int>(up) - kMostUp;
+        if (__builtin_expect(wide_range, 0)) {
+            float reach = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            y[j] = gone >> j & 1u ? 0.0f : w[j];  // (0 times a scale that is no number)
-            most = fmaxf(most, fabsf(y[j]) < INFINITY ? fabsf(y[j]) : 0.0f);
+            for (int j = 0; j < 16; ++j) {
+                w[j] = gone >> j & 1u ? 0.0f : w[j];  // (0 times a scale that is no number)
+                most = fmaxf(most, fabsf(w[j]) < INFINITY ? fabsf(w[j]) : 0.0f);
+            }
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) reach = fmaxf(reach, fabsf(acc[i][j]) < INFINITY ? fabsf(acc[i][j]) : 0.0f);
+            reach = fmaxf(reach, butterfly_partner<32>(reach, lane));
+            least = static_cast<int>(up) - 126;
+            if (reach > 0) least = max(least, __builtin_amdgcn_frexp_expf(reach) - 125);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(w[j]));
         }
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) sum = fmaxf(sum, fabsf(acc[i][j]) < INFINITY ? fabsf(acc[i][j]) : 0.0f);
         most = fmaxf(most, butterfly_partner<32>(most, lane));
-        sum = fmaxf(sum, butterfly_partner<32>(sum, lane));
-        int unit = most > 0 ? max(-126, __builtin_amdgcn_frexp_expf(most) - 10) : 0;
-        if (sum > 0) unit = max(unit, __builtin_amdgcn_frexp_expf(sum) - 100);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            float z[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] = ldexpf(y[8 * ks + j], -unit);
-            p[ks] = halve8_any(z);
-        }
+        const int unit = max(least, most > 0 ? __builtin_amdgcn_frexp_expf(most) - 10 : 0);
         const float to = ldexpf(1.0f, -unit);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] *= to;
 #pragma unroll
         for (int i = 0; i < DT; ++i) acc[i] *= to;
         return unit;
@@ -442,15 +453,22 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
         top = fmaxf(top, butterfly_partner<32>(top, lane)) * down;
         const int follow = max(-kMostExp, min(kMostExp, ve));
         const float high = ceilf(top) + static_cast<float>(max(-kMostExp, min(kMostExp, ve)));
-        if (__any(high > M + kSlack)) {  // (above M = -inf: the first scores)
+        float up = 0.0f;
+        bool low = false;
+        // (M = -inf: the first scores; rows that attend none of the tile are here too)
+        if (__any(fabsf(high - M + 0.5f * (kDrop - kSlack)) > 0.5f * (kDrop + kSlack))) {
             const float most = fmaxf(M, high);
             const float alpha = M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - most);
             M = most;
-            l *= alpha;
+            const bool below = high < M - kDrop && high > -INFINITY && !wide_range;
+            low = __any(below);
+            up = below ? fminf(M - high, static_cast<float>(kMostUp)) : 0.0f;
+            const float grow = alpha * __builtin_amdgcn_exp2f(up);
+            l *= grow;
 #pragma unroll
-            for (int i = 0; i < DT; ++i) acc[i] *= alpha;
+            for (int i = 0; i < DT; ++i) acc[i] *= grow;
         }
-        const float lifted = M > -INFINITY ? kLift - M : 0.0f;  // nothing attended yet: every power is 0
+        const float lifted = M > -INFINITY ? kLift + up - M : 0.0f;  // nothing attended yet: every power is 0
         // the next tile's product beside this tile's weights (ahead of the other block's wave: 466 -> 456 us where the
         // matrix unit is the bound)
         __builtin_amdgcn_s_setprio(1);
@@ -468,20 +486,35 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
             l += (p[0] + p[1]) + (p[2] + p[3]);
         }
         Halves p[2];
+        auto halve = [&] {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            float w[8];
+            for (int ks = 0; ks < 2; ++ks) {
+                float w[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = x[8 * ks + j];
-            p[ks] = halve8(w);
-        }
+                for (int j = 0; j < 8; ++j) w[j] = x[8 * ks + j];
+                p[ks] = halve8(w);
+            }
+        };
+        halve();
         // a row none of whose weights reaches 2 (the first bit of a float16 exponent), though it attends some of the keys
         const uint32_t bits = (p[0].hi.x | p[0].hi.y | p[0].hi.z | p[0].hi.w) | (p[1].hi.x | p[1].hi.y | p[1].hi.z | p[1].hi.w);
         const uint64_t held = __ballot((bits & 0x40004000u) != 0);
-        const bool apart =
-            code > kMostExp || (static_cast<uint32_t>(held) | static_cast<uint32_t>(held >> 32) | idle) != ~0u;
-        int unit = 0;
-        if (apart) unit = rescale(p, x, gone);
+        const bool far = code > kMostExp;
+        const bool apart = far || (static_cast<uint32_t>(held) | static_cast<uint32_t>(held >> 32) | idle) != ~0u;
+        int back = static_cast<int>(-up);
+        if (__builtin_expect(apart, 0)) {
+            back += rescale(x, gone, far, up);
+            halve();
+            if (__builtin_expect(far, 0)) {
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    float w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j] = x[8 * ks + j];
+                    p[ks] = halve8_any(w);
+                }
+            }
+        }
         // this tile's values beside the operands of the tiles to come
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -493,8 +526,9 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
         place_v(rv_next, tile + 1);
         place_k(rk_next, tile + 2);
         __builtin_amdgcn_s_setprio(0);
-        if (apart) {
-            const float from = ldexpf(1.0f, unit);
+        if (__builtin_expect(apart || low, 0)) {
+            l *= __builtin_amdgcn_exp2f(-up);
+            const float from = ldexpf(1.0f, back);
 #pragma unroll
             for (int i = 0; i < DT; ++i) acc[i] *= from;
         }

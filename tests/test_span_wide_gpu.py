@@ -355,6 +355,23 @@ def test_v_scales_that_change_from_tile_to_tile(hd):
     piece(rng, hd, change, tokens=(0, 39))
 
 
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("at", [0, 40, 170, 299])
+@pytest.mark.parametrize("margin", [12, 40, 60])
+def test_scores_far_apart_and_v_scales_that_change(hd, at, margin):
+    """A slot with scores far ahead, in an early or late tile, whose V row has zeros in half of the dimensions, beside tiles
+    of V scales far above and below: tiles far below the row's maximum with scales beyond what it follows."""
+    rng = np.random.default_rng(hd + at + margin)
+    q = queries(rng, PIECE, hd)
+
+    def change(r):
+        dominant(q, r, at, margin)
+        r.v[:, at, :, ::2] = 0
+        for t, e in enumerate((0, 55, -20, 3, 70, -3, 8, -8, 60, 0, 20)):
+            r.vs[:, 32 * t:32 * t + 32] *= np.float32(2.0 ** e)
+    piece(rng, hd, change, q, tokens=(0, 1, 39))
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("apart", [12, 24, 36])
 def test_prefix_the_largest_score_at_a_small_v_scale(hd, apart):

@@ -12,10 +12,11 @@
 //   one's that the row does not attend; or the scores are far below the row's largest), the tile is added with a power of
 //   two of its own a row, whose largest is then in [2^9, 2^10). V rows of zeros as the cache stores them (scale 1) count
 //   for none of this. Held in fp32 before that, a weight below 2^-119 of the row's largest V scale may be lost.
-// 6 x 999 tokens, 32 heads of 128 values, window 2048: 428 us, 1.0 PFLOP/s of matrix work (a large bfloat16 product of the
-// library reaches 1.2). The matrix unit is busy 47% of the cycles; the rest is the softmax and the making of terms, 258
-// vector instructions a wave and tile next to its 32 matrix instructions. Rows of 64: 362 us. A third block a
-// compute unit spills.
+// 6 x 999 tokens, 32 heads of 128 values, window 2048, rows stored before: 435 us a call, 428 GFLOP of matrix work at
+// 0.98 PFLOP/s (a large bfloat16 product of the library reaches 1.2); rows of 64 305 us, of 32 197. The matrix unit is busy
+// 45% of the cycles; the rest is the softmax and the making of terms, 256 vector instructions a wave and tile next to its 32
+// matrix instructions. Tiles with powers of two of their own: peaky scores (three times these) 510 us, rows of 64 345.
+// Two blocks a compute unit: with rows of 128 up to 10 registers are kept in memory around the loop over tiles, none in it.
 #include "span_rows.h"
 
 namespace nd {

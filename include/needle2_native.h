@@ -303,8 +303,12 @@ int needle2_gpu_kv_export(void *kv, int layer, int seq, int8_t *k, int8_t *v, fl
  * read on the host, so every call can be captured once it has run with the
  * same sizes (its scratch belongs to the handle, is never moved while the
  * handle lives, and is not for two calls at once). The handle must have been
- * made on the current device. A head without a softmax (no slot to attend, a
- * non-finite query) yields zeros, as in needle2_gpu_attention. All return
+ * made on the current device. Sums are fp32. Where many query rows attend the
+ * same slots (prompt pieces, a batch's prefix) a value of a query and a weight
+ * times its V scale are held to 2^-23 of themselves, and such a weight to 2^-26
+ * of the row's largest among 32 slots if that is more; else both are exact. A
+ * head without a softmax (no slot to attend, a non-finite query) yields zeros,
+ * as in needle2_gpu_attention. All return
  * 0 / -1 (message in needle2_gpu_error); a refused call does nothing. */
 
 /* Attention of `count` consecutive new tokens per sequence over a window with

@@ -2,10 +2,10 @@
 // prefix. The mathematics and the records are span_kernels.hip's. The matrix instructions bound this kernel, so both
 // products run on v_mfma_f32_32x32x16_f16 with q and p * vs as two float16 terms (the codes are float16 numbers as they
 // are) instead of three bfloat16 ones: 22 bits of a value, and of small values what lies above 2^-25 of the term's unit.
-//   q is scaled by a power of two so that the row's largest |q| is in [2^14, 2^15). Of a value the terms leave at most
-//   2^-23 (the last bit of a quarter of them; the sums round by as much), of a small one at most 2^-25, together
-//   2^-25 * 127 HD * |ks| in a score; where that could pass 2^-24 (of a score times log2 e, whose own rounding is 2^-24 of its
-//   size) the tile's scores get the rest of q in further terms, until nothing is left.
+//   q is scaled by a power of two, 2^kMostLift at most, so that the row's largest |q| is in [2^14, 2^15). Of a value the
+//   terms leave at most 2^-23 (the last bit of a quarter of them; the sums round by as much), of a small one at most 2^-25,
+//   together 2^-25 * 127 HD * |ks| in a score; where that could pass 2^-24 (of a score times log2 e, whose own rounding is
+//   2^-24 of its size) the tile's scores get the rest of q in further terms, until nothing is left.
 //   p * vs is scaled by one power of two a row, 2^(kLift - M), that follows the largest score and the largest V scale, and of
 //   it the terms leave at most 2^-23, of a small one 2^-25: 2^-26 of the row's largest in the tile, where that is at least 2
 //   (an fp32 sum of the 32 rounds by 2^-24 of its largest term). Where it is not (the largest V scale is another key's, or
@@ -108,6 +108,9 @@ __device__ __forceinline__ u32x4 widen_half(uint32_t a, uint32_t b) {
 constexpr float kLift = 10.0f, kSlack = 5.0f, kDrop = 7.0f;
 constexpr int kMostExp = 50;  // of a V scale that M follows: the sum, which M scales too, stays far from underflow
 constexpr int kMostUp = 76;
+// of q: scores, held times 2^lift, stay finite up to 2^97 (smaller q lie below the terms; where their scores could matter
+// they are taken in further ones)
+constexpr int kMostLift = 30;
 constexpr int kOddTile = 1024;
 
 constexpr int kFrag = 66;  // 16-byte lanes of an operand in LDS: 32, one of padding (the halves in different banks), 32, 1
@@ -298,7 +301,7 @@ __device__ __forceinline__ void span_wide(const SpanArgs &a, int bx) {
         }
         most = fmaxf(most, butterfly_partner<32>(most, lane));
         finite = butterfly_partner<32>(finite ? 1.0f : 0.0f, lane) != 0.0f && finite;
-        lift = finite && most > 0 ? min(15 - __builtin_amdgcn_frexp_expf(most), 120) : 0;
+        lift = finite && most > 0 ? min(15 - __builtin_amdgcn_frexp_expf(most), kMostLift) : 0;
         down = finite ? ldexpf(1.0f, -lift) : __builtin_nanf("");
         worst = wave_max(finite && most > 0 ? down : 0.0f, lane) * (127.0f * HD * 0.5f);
 #pragma unroll

@@ -130,6 +130,22 @@ def test_uneven_queries(hd, ratio):
 
 
 @pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("apart", [-110, -60, 20, 60, 90, 110])
+@pytest.mark.parametrize("margin", [0, 30000])
+def test_extreme_queries_and_k_scales(hd, apart, margin):
+    """Queries 2^apart times smaller, K scales as much larger; a slot with scores of 30000."""
+    rng = np.random.default_rng(hd + apart + 200)
+    q = queries(rng, PIECE, hd)
+
+    def change(r):
+        if margin:
+            dominant(q, r, 77, margin)
+        r.ks *= np.float32(2.0 ** apart)
+        q[:] *= np.float32(2.0 ** -apart)
+    piece(rng, hd, change, q, tokens=(0, 1, 39))
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
 @pytest.mark.parametrize("margin", [3, 10, 30, 60, 120])
 def test_dominant_slots(hd, margin):
     """Some slots whose scores are `margin` above the rest, with zero V codes in half of the dimensions: there the other

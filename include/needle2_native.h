@@ -241,7 +241,8 @@ int needle2_gpu_device_info(char *buf, int len);         /* "name;arch;cus;hbm_b
  * what is issued to `stream` between begin and end, instantiate, replay with
  * one launch. Entry points used inside must have run once before the capture
  * and must not read host memory: plan_run, attention (all forms),
- * kv_store_device, kv_evict. */
+ * and must not read host memory: plan_run, attention (all forms),
+ * kv_store_device, kv_evict, pages_* (but pages_free) and heads*. */
 int needle2_gpu_graph_begin(void *stream);
 void *needle2_gpu_graph_end(void *stream);                /* instantiated graph, or NULL */
 int needle2_gpu_graph_launch(void *graph, void *stream);
@@ -360,6 +361,89 @@ int needle2_gpu_kv_evict(void *kv, int layer, const float *d_weights, const int 
 /* Device addresses of a layer's rows: codes [seqs][kvheads][capacity][head_dim]
  * and fp32 scales [seqs][kvheads][capacity], valid while the handle lives. */
 int needle2_gpu_kv_layer(void *kv, int layer, int8_t **d_k, int8_t **d_v, float **d_k_scales, float **d_v_scales);
+
+/* ---- a paged int8 cache for many requests -------------------------------------
+ * The reference holds one sequence in one run of slots
+ * (needle2/csrc/engine.cpp:433-449); here requests of any length share `pages`
+ * pages of page_size positions (16, 32, 64, 128 or 256) each. A layer holds, for
+ * page p and kv head h, block p * kvheads + h: the positions' K codes
+ * [page_size][head_dim], V codes, K scales [page_size] and V scales, codes and
+ * scales as in the cache above. Slot s is position s % page_size of page
+ * s / page_size. d_tables (device int32 [requests][width]) has the pages of every
+ * request's positions in order; a page outside [0, pages) is none. Nothing is
+ * read on the host, except by pages_free, so every call can be captured once it
+ * has run with the same sizes. The handle must have been made on the current
+ * device; its calls must not overlap in time (they share its free pages and its
+ * scratch, which never moves while the handle lives). At most 8192 requests and
+ * 2^25 tokens a call, width * page_size at most 2^30. All return 0 / -1 (message
+ * in needle2_gpu_error); a refused call does nothing. */
+void *needle2_gpu_pages_create(int layers, int pages, int page_size, int kvheads, int head_dim);
+void needle2_gpu_pages_destroy(void *cache);
+size_t needle2_gpu_pages_storage_bytes(void *cache);
+/* Device address of a layer's blocks, valid while the handle lives. */
+int needle2_gpu_pages_layer(void *cache, int layer, uint8_t **d_rows);
+/* Number of free pages once `stream` has run what it has (waits for it). */
+int needle2_gpu_pages_free(void *cache, int *count, void *stream);
+/* All pages are free again; tables made before are not to be used any more. */
+int needle2_gpu_pages_reset(void *cache, void *stream);
+/* Pages for counts[r] (negative: 0) new tokens of every request r that holds
+ * lengths[r] positions, dealt request by request and page by page: written into
+ * d_tables, and d_lengths advanced. The requests' tokens lie one after the other
+ * in a batch of at most `tokens`: d_starts ([requests + 1]) has where each one's
+ * begin, and where the last one's end; d_firsts ([requests]) the position of its
+ * first; d_positions and d_slots ([tokens]) every token's. A request whose tokens
+ * pass its table or the batch, or that comes where the free pages no longer
+ * suffice, gets none: its length stays, its first position is -1, and so are its
+ * tokens' positions and slots, as are those behind the last request's. (One that
+ * needs no new page is served all the same.) */
+int needle2_gpu_pages_extend(void *cache, int requests, const int *d_counts, int tokens, int *d_lengths, int *d_tables,
+                             int width, int *d_starts, int *d_firsts, int *d_slots, int *d_positions, void *stream);
+/* Cuts request r to its first keep[r] positions (negative: 0; not longer than it
+ * is): d_lengths is lowered, and the pages that hold none of them are free again
+ * and -1 in d_tables. Right after an extension, a trim to the lengths before it
+ * undoes it. Tables that hold pages which another request's table has too, or
+ * that no extension dealt, are not for this call. */
+int needle2_gpu_pages_trim(void *cache, int requests, const int *d_keep, int *d_lengths, int *d_tables, int width,
+                           void *stream);
+/* d_k, d_v: device fp32 rows [tokens], k_stride and v_stride floats from one to
+ * the next (multiples of 4, rows at multiples of 16 bytes), kvheads * head_dim
+ * each; token i goes to slot d_slots[i]; a slot outside the cache: not stored.
+ * No two tokens have the same slot. */
+int needle2_gpu_pages_store(void *cache, int layer, const float *d_k, int k_stride, const float *d_v, int v_stride,
+                            int tokens, const int *d_slots, void *stream);
+/* Norms and rotation of the heads of q and k, as in Engine::step
+ * (needle2/csrc/engine.cpp:994-1004) for a batch of tokens: where a gain
+ * ([head_dim], nullable: not normed) is set, a head x becomes
+ * x / sqrt(mean(x^2) + eps) * (1 + gain); then dimensions j and j + rotary / 2 are
+ * turned by d_positions[token] * d_freq[j] (device fp64 [rotary / 2]; rotary 0:
+ * not at all). head_dim 32, 64 or 128. Rows as in pages_store, of heads * head_dim
+ * and kvheads * head_dim (0: none); outputs in place (the same stride) or apart.
+ * A token at a negative position (d_positions nullable without a rotation) is left
+ * out, its outputs as they were. */
+int needle2_gpu_heads(const float *d_q, int q_stride, float *d_q_out, int q_out_stride, int heads, const float *d_k,
+                      int k_stride, float *d_k_out, int k_out_stride, int kvheads, int head_dim, int tokens,
+                      const int *d_positions, const float *d_q_gain, const float *d_k_gain, float eps, const double *d_freq,
+                      int rotary, void *stream);
+/* needle2_gpu_heads that also stores the k rows it makes, and v's, in d_slots (as
+ * pages_store of its results), in the same launch; d_k_out may be NULL. */
+int needle2_gpu_heads_store(void *cache, int layer, const float *d_q, int q_stride, float *d_q_out, int q_out_stride,
+                            int heads, const float *d_k, int k_stride, float *d_k_out, int k_out_stride, const float *d_v,
+                            int v_stride, int tokens, const int *d_positions, const int *d_slots, const float *d_q_gain,
+                            const float *d_k_gain, float eps, const double *d_freq, int rotary, void *stream);
+/* Attention of a ragged batch of new tokens, stored already. d_q, d_out: device
+ * fp32 [tokens][heads][head_dim], at multiples of 16 bytes; request r has rows
+ * d_starts[r] .. d_starts[r + 1] - 1 (at most the first `count` of them are
+ * attended), the first at position d_firsts[r]; a token attends every position of
+ * its request up to its own, or the last `window` of them (0: all). A request at a
+ * negative first position, or whose tokens pass its table, yields zeros; positions
+ * of no page are not attended. Rows of no request are left as they were. heads: a
+ * multiple of kvheads, 1 to 16 per kv head; at most 2^25 query rows. length: the
+ * most positions that a request has (0: unknown): how the work is cut goes by it,
+ * the results do not depend on it. Exactness, and heads without a softmax, as
+ * described above for long contexts. */
+int needle2_gpu_pages_attention(void *cache, int layer, const float *d_q, float *d_out, int heads, int requests, int tokens,
+                                int count, const int *d_starts, const int *d_firsts, const int *d_tables, int width,
+                                int length, int window, void *stream);
 
 #ifdef __cplusplus
 }

@@ -10,8 +10,10 @@ repository's own interface to it:
 - ``cq``      CQ matrices (FP32 and int8 products, rows, candidates, the
               prefill GEMM) and multi-matrix plans;
 - ``kv``      the int8 KV cache of a decode batch and its attention;
+- ``paged``   the int8 KV cache in pages, for requests of different lengths;
+- ``heads``   norms and rotation of the heads of q and k;
 - ``engine``  the single-sequence decode engine;
 - ``archive`` / ``formats``  the ``.cact`` file and the CQ storage format.
 """
 
-__all__ = ["archive", "cq", "device", "engine", "formats", "kv"]
+__all__ = ["archive", "cq", "device", "engine", "formats", "heads", "kv", "paged"]

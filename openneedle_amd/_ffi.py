@@ -111,6 +111,19 @@ SIGNATURES: dict[str, tuple] = {
     "needle2_gpu_attention_weights": (i32, [vp, i32, vp, vp, vp, i32, i32, vp, vp, vp, vp]),
     "needle2_gpu_kv_evict": (i32, [vp, i32, vp, vp, i32, i32, i32, vp, vp, vp, vp]),
     "needle2_gpu_kv_layer": (i32, [vp, i32, vp, vp, vp, vp]),
+    "needle2_gpu_pages_create": (vp, [i32, i32, i32, i32, i32]),
+    "needle2_gpu_pages_destroy": (None, [vp]),
+    "needle2_gpu_pages_storage_bytes": (sz, [vp]),
+    "needle2_gpu_pages_layer": (i32, [vp, i32, vp]),
+    "needle2_gpu_pages_free": (i32, [vp, vp, vp]),
+    "needle2_gpu_pages_reset": (i32, [vp, vp]),
+    "needle2_gpu_pages_extend": (i32, [vp, i32, vp, i32, vp, vp, i32, vp, vp, vp, vp, vp]),
+    "needle2_gpu_pages_trim": (i32, [vp, i32, vp, vp, vp, i32, vp]),
+    "needle2_gpu_pages_store": (i32, [vp, i32, vp, i32, vp, i32, i32, vp, vp]),
+    "needle2_gpu_heads": (i32, [vp, i32, vp, i32, i32, vp, i32, vp, i32, i32, i32, i32, vp, vp, vp, f32, vp, i32, vp]),
+    "needle2_gpu_heads_store": (i32, [vp, i32, vp, i32, vp, i32, i32, vp, i32, vp, i32, vp, i32, i32, vp, vp, vp, vp, f32,
+                                      vp, i32, vp]),
+    "needle2_gpu_pages_attention": (i32, [vp, i32, vp, vp, i32, i32, i32, i32, vp, vp, vp, i32, i32, i32, vp]),
 }
 
 

@@ -1,0 +1,53 @@
+// gfx950 kernels of attention over the paged cache: new tokens of many requests, one, a draft or a prompt piece each. The
+// mathematics, the operands and the records are span_kernels.hip's; a tile's pages are looked up ahead of its loads.
+#include "paged.h"
+#include "span_join.h"
+#include "span_rows.h"
+
+namespace nd {
+
+namespace {
+
+template <int HD, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void paged_kernel(PagedSpanArgs a) {
+    span_block<HD, NW, Keys::Paged>(a, blockIdx.x);
+}
+
+template <int HD, int G>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedSpanArgs a, int64_t rows) {
+    constexpr int kRows = 256 / (G * (HD / 4));
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
+    join_rows<HD, G, true>(a, row0, static_cast<int>(min(static_cast<int64_t>(kRows), rows - row0)), a.records);
+}
+
+template <int HD>
+void launch_hd(const PagedSpanArgs &a, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.splits) * a.row_tiles * a.kvheads * a.units));
+    if (a.waves == 4) hipLaunchKernelGGL((paged_kernel<HD, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((paged_kernel<HD, 8>), grid, dim3(512), 0, s, a);
+    ND_HIP(hipGetLastError());
+}
+
+}  // namespace
+
+void launch_paged(const PagedSpanArgs &a, int head_dim, hipStream_t s) {
+    switch (head_dim) {
+    case 32: launch_hd<32>(a, s); break;
+    case 64: launch_hd<64>(a, s); break;
+    default: launch_hd<128>(a, s); break;
+    }
+}
+
+void launch_paged_join(const PagedSpanArgs &a, int head_dim, hipStream_t s) {
+    ND_CHECK(a.splits_total <= kJoinMax, "attention: too many pieces");
+    const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
+    with_join(head_dim, a.splits_total, [&](auto hd, auto groups) {
+        constexpr int HD = decltype(hd)::value, G = decltype(groups)::value;
+        constexpr int kRows = 256 / (G * (HD / 4));
+        hipLaunchKernelGGL((paged_join_kernel<HD, G>), dim3(static_cast<unsigned>((rows + kRows - 1) / kRows)), dim3(256), 0,
+                           s, a, rows);
+    });
+    ND_HIP(hipGetLastError());
+}
+
+}  // namespace nd

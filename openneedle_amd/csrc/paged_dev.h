@@ -1,0 +1,57 @@
+// What the attention kernels read through a page table.
+#pragma once
+
+#include "paged.h"
+
+namespace nd {
+
+// Memory that no kernel of the running launch writes, read through the scalar cache where the address is uniform.
+#define ND_CONST __attribute__((address_space(4)))
+
+// A request's tokens: the first one's row of q and its position, and how many. A request that does not lie in its table (or
+// at a negative position) attends nothing.
+struct Request {
+    int token, count, first;
+};
+__device__ __forceinline__ Request request(const PagedSpanArgs &a, int r) {
+    const ND_CONST int *starts = (const ND_CONST int *)(a.starts), *firsts = (const ND_CONST int *)(a.positions);
+    const int t0 = max(0, min(starts[r], a.tokens)), t1 = max(t0, min(starts[r + 1], a.tokens));
+    Request q = {t0, min(t1 - t0, a.count), firsts[r]};
+    if (q.first < 0 || q.first > (a.width << a.pool.shift) - q.count) q.first = -1;
+    return q;
+}
+
+// The pages of a request and kv head. A page outside the cache is none (-1): its rows read as zeros and are masked.
+template <int HD>
+struct PageReader {
+    const ND_CONST int *table;
+    const uint8_t *at;
+    size_t page_bytes;  // of all kv heads
+    int width, pages, shift;
+    __device__ __forceinline__ PageReader() = default;
+    __device__ __forceinline__ PageReader(const PagedSpanArgs &a, int unit, int kh)
+        : table((const ND_CONST int *)(a.tables + static_cast<size_t>(unit) * a.width)),
+          at(a.pool.at + static_cast<size_t>(kh) * page_block_bytes(a.pool.shift, HD)),
+          page_bytes(static_cast<size_t>(a.pool.kvheads) * page_block_bytes(a.pool.shift, HD)), width(a.width),
+          pages(a.pool.pages), shift(a.pool.shift) {}
+    __device__ __forceinline__ int id(int position) const {
+        const int i = position >> shift;
+        const int p = table[min(i, width - 1)];
+        return i < width && static_cast<unsigned>(p) < static_cast<unsigned>(pages) ? p : -1;
+    }
+    __device__ __forceinline__ const uint8_t *block(int id) const { return at + max(id, 0) * page_bytes; }
+    __device__ __forceinline__ int off(int position) const { return position & ((1 << shift) - 1); }
+    // 16 rows from a position on (a multiple of 16); past them, and of no page, zeros
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t k_codes(int id, int position) const {
+        return buffer_rsrc(block(id) + off(position) * HD, id >= 0 ? 16 * HD : 0);
+    }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t v_codes(int id, int position) const {
+        return buffer_rsrc(block(id) + (HD << shift) + off(position) * HD, id >= 0 ? 16 * HD : 0);
+    }
+    // their K scales; the V scales are 1 << shift further
+    __device__ __forceinline__ const float *k_scales(int id, int position) const {
+        return reinterpret_cast<const float *>(block(id) + (2 * HD << shift)) + off(position);
+    }
+};
+
+}  // namespace nd

@@ -50,6 +50,20 @@ ND_BOTH KeyRuns ring_runs(int first, int last, int sinks, int window, int capaci
     return r;
 }
 
+// Queries at positions first .. last over positions themselves (a page table says where each lies): one run from a whole
+// number of tiles on, so that a tile has whole pieces of 16 positions. What lies before the window is masked.
+ND_BOTH KeyRuns page_runs(int first, int last, int window, int tile) {
+    KeyRuns r = {0, 0, 0, 0, 0, 0};
+    if (first < 0) return r;
+    const int low = window > 0 && first >= window ? first - window + 1 : 0;
+    r.begin1 = low / tile * tile;
+    r.n1 = last + 1 - r.begin1;
+    return r;
+}
+
+// What the kernels attend: slots [0, n) of a unit; a ring with pinned first positions; positions through a page table.
+enum class Keys { Flat, Ring, Paged };
+
 constexpr int kSpanTile = 64;  // keys of a tile; a tile lies in one run
 
 constexpr int kWideTile = 32;  // where many query rows share them

@@ -9,6 +9,7 @@
 //
 // Both products run on v_mfma_f32_16x16x32_bf16. The codes are bfloat16 numbers as they are; q and p * vs are three
 // bfloat16 terms each (8 + 8 + 8 bits: the fp32 value exactly, at any magnitude), so only the sums round, in fp32.
+#include "span_join.h"
 #include "span_rows.h"
 
 #include <cmath>
@@ -47,98 +48,17 @@ __global__ __launch_bounds__(256) void span_store_kernel(SpanStoreArgs a) {
     if (part == 0) (values ? a.c.vs : a.c.ks)[row] = top > 0 ? top / 127.0f : 1.0f;
 }
 
-template <int HD, int NW, bool RING>
+template <int HD, int NW, Keys K>
 __global__ __launch_bounds__(64 * NW, 2) void span_kernel(SpanArgs a) {
-    span_block<HD, NW, RING>(a, blockIdx.x);
+    span_block<HD, NW, K>(a, blockIdx.x);
 }
 
 // A shared prefix and the units' own keys in one launch: the first `far_blocks` blocks have the prefix.
 template <int HD, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void span_two_kernel(SpanArgs far, SpanArgs own, int far_blocks) {
     const int b = blockIdx.x;
-    if (b < far_blocks) span_block<HD, NW, false>(far, b);
-    else span_block<HD, NW, false>(own, b - far_blocks);
-}
-
-// A row's maximum and sum over its records, by one wave; the records' factors 2^(m - maximum) to `factor` if that is set.
-__device__ __forceinline__ float2 join_sums(const SpanArgs &a, size_t row, int lane, float *factor) {
-    const float2 *ml = a.rec_ml + row * a.splits_total;
-    float2 mine = make_float2(-INFINITY, 0.0f);  // of this lane's first record: most rows have no second
-    float M = -INFINITY;
-    for (int s = lane; s < a.splits_total; s += 64) {
-        const float2 v = ml[s];
-        if (s == lane) mine = v;
-        M = fmaxf(M, v.x);
-    }
-    M = wave_max(M, lane);
-    const float base = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f;
-    for (int s = lane; s < a.splits_total; s += 64) {
-        const float2 v = s == lane ? mine : ml[s];
-        const bool empty = v.x == -INFINITY && v.y == 0.0f;
-        const float f = empty ? 0.0f : __builtin_amdgcn_exp2f(v.x - base);
-        if (factor) factor[s] = f;
-        L += empty ? 0.0f : f * v.y;
-    }
-    return make_float2(base, wave_sum(L, lane));
-}
-
-// Rows row0 .. row0 + count - 1 from their records, by a block of 256: G groups of HD / 4 lanes share a row's records
-// (every G-th each), whose loads do not wait for each other; 256 / (G * HD / 4) rows at a time. The sums' order depends
-// on the number of records only. Latency bounds it: 64 x 32 rows of 128 values 5 us, a long prefix's many records 7.
-constexpr int kJoinMax = 1024;  // records of a row
-template <int HD, int G>
-__device__ __forceinline__ void join_rows(const SpanArgs &a, size_t row0, int count) {
-    constexpr int kLanes = HD / 4, kRows = 256 / (G * kLanes);
-    constexpr int kFactors = kRows * (G == 8 ? kJoinMax : G);
-    __shared__ float factor[kFactors];
-    __shared__ float total[kRows];
-    __shared__ __attribute__((aligned(16))) float part[G > 1 ? G : 1][kRows][HD];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int splits = a.splits_total;
-    const int d = t % kLanes * 4, g = t / kLanes % G, r = t / (kLanes * G);
-    for (int i0 = 0; i0 < count; i0 += kRows) {
-        for (int i = wave; i < kRows && i0 + i < count; i += 4) {
-            const float2 all = join_sums(a, row0 + i0 + i, lane, factor + i * splits);
-            if (lane == 0) total[i] = all.y;
-        }
-        __syncthreads();
-        const bool live = i0 + r < count;
-        float4 o = make_float4(0, 0, 0, 0);
-        if (live) {
-            const float *rec = a.rec_o + (row0 + i0 + r) * splits * HD + d;
-#pragma unroll 4
-            for (int s = g; s < splits; s += G) {
-                const float f = factor[r * splits + s];
-                const float4 p = *reinterpret_cast<const float4 *>(rec + static_cast<size_t>(s) * HD);
-                if (f == 0.0f) continue;  // an empty piece, or weights that vanish beside the rest
-                o.x = __builtin_fmaf(f, p.x, o.x);
-                o.y = __builtin_fmaf(f, p.y, o.y);
-                o.z = __builtin_fmaf(f, p.z, o.z);
-                o.w = __builtin_fmaf(f, p.w, o.w);
-            }
-        }
-        if constexpr (G > 1) {
-            *reinterpret_cast<float4 *>(&part[g][r][d]) = o;
-            __syncthreads();
-            if (g == 0) {
-#pragma unroll
-                for (int k = 1; k < G; ++k) {
-                    const float4 p = *reinterpret_cast<const float4 *>(&part[k][r][d]);
-                    o.x += p.x;
-                    o.y += p.y;
-                    o.z += p.z;
-                    o.w += p.w;
-                }
-            }
-        }
-        if (live && g == 0) {
-            const float L = total[r], inv = 1.0f / L;
-            *reinterpret_cast<float4 *>(a.out + (row0 + i0 + r) * HD + d) =
-                L > 0 ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0, 0, 0, 0);
-        }
-        __syncthreads();
-    }
+    if (b < far_blocks) span_block<HD, NW, Keys::Flat>(far, b);
+    else span_block<HD, NW, Keys::Flat>(own, b - far_blocks);
 }
 
 template <int HD, int G>
@@ -176,7 +96,7 @@ __global__ __launch_bounds__(256) void span_record_kernel(SpanRecordArgs r) {
             ahead[g][u] = in[u] && g < a.group ? x[static_cast<size_t>(g) * a.score_stride + 256 * u] : 0.0f;
     }
     for (int g = t >> 6; g < a.group; g += 4) {
-        const float2 v = join_sums(a, row0 + g, t & 63, nullptr);
+        const float2 v = join_sums(a, row0 + g, a.splits_total, t & 63, nullptr);
         if ((t & 63) == 0) all[g] = v;
     }
     __syncthreads();
@@ -243,31 +163,11 @@ void launch_span(const SpanArgs &a, int head_dim, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(a.splits * row_tiles(a) * a.kvheads * a.units));
     with_rows(head_dim, a.waves, [&](auto hd, auto waves) {
         constexpr int HD = decltype(hd)::value, NW = decltype(waves)::value;
-        if (a.positions) hipLaunchKernelGGL((span_kernel<HD, NW, true>), grid, dim3(64 * NW), 0, s, a);
-        else hipLaunchKernelGGL((span_kernel<HD, NW, false>), grid, dim3(64 * NW), 0, s, a);
+        if (a.positions) hipLaunchKernelGGL((span_kernel<HD, NW, Keys::Ring>), grid, dim3(64 * NW), 0, s, a);
+        else hipLaunchKernelGGL((span_kernel<HD, NW, Keys::Flat>), grid, dim3(64 * NW), 0, s, a);
     });
     ND_HIP(hipGetLastError());
 }
-
-namespace {
-
-// F(head_dim, groups that share a row's records)
-template <class F>
-void with_join(int head_dim, int splits, F &&f) {
-    auto groups = [&](auto hd) {
-        if (splits <= 1) f(hd, std::integral_constant<int, 1>{});
-        else if (splits <= 2) f(hd, std::integral_constant<int, 2>{});
-        else if (splits <= 4) f(hd, std::integral_constant<int, 4>{});
-        else f(hd, std::integral_constant<int, 8>{});
-    };
-    switch (head_dim) {
-    case 32: groups(std::integral_constant<int, 32>{}); break;
-    case 64: groups(std::integral_constant<int, 64>{}); break;
-    default: groups(std::integral_constant<int, 128>{}); break;
-    }
-}
-
-}  // namespace
 
 void launch_span_join(const SpanArgs &a, int head_dim, hipStream_t s) {
     ND_CHECK(a.splits_total <= kJoinMax, "attention: too many pieces");

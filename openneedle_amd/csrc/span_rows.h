@@ -2,6 +2,7 @@
 // mathematics).
 #pragma once
 
+#include "paged_dev.h"
 #include "span_dev.h"
 
 namespace nd {
@@ -22,8 +23,11 @@ __device__ __forceinline__ f32x4 mfma(const u32x4 &a, const u32x4 &b, const f32x
 //   Values: operand B is p * vs straight from those registers (the contraction runs over the keys in their order:
 //   depth 8 (l / 16) + j is key 32 u + 4 (l / 16) + j, and from j = 4 on 32 u + 16 + 4 (l / 16) + j - 4), operand A the V
 //   codes of dimensions HD / 16 * (l % 16) + t. Result t of lane l is row l % 16, dimensions HD / 16 * (4 (l / 16) + i) + t.
-template <int HD, int NW, bool RING>
-__device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int unit) {
+// Paged: the unit is a request of its own number of tokens, row tile and piece are `bx`; its keys are cut into as many
+// pieces as there are tiles for, at most `splits` of at least `per` tiles.
+template <int HD, int NW, Keys K, class A>
+__device__ __forceinline__ void span_rows(const A &a, int bx, int kh, int unit) {
+    constexpr bool RING = K == Keys::Ring, PAGED = K == Keys::Paged;
     constexpr int kSteps = HD / 32;        // of the score product's depth
     constexpr int kBytes = HD / 4;         // of a K row per lane
     constexpr int VB = HD / 16;            // bytes of a V row per lane
@@ -33,9 +37,16 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
 
     const int t = threadIdx.x, lane = t & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int tiles_of_rows = (a.count * a.group + kSpanRows - 1) / kSpanRows;
+    int tiles_of_rows = (a.count * a.group + kSpanRows - 1) / kSpanRows;
+    int rows = a.count * a.group;
+    Request req;
+    if constexpr (PAGED) {
+        tiles_of_rows = a.row_tiles;
+        req = request(a, unit);
+        rows = req.count * a.group;
+        if (bx % tiles_of_rows * kSpanRows >= rows || rows > a.small) return;
+    }
     const int tile0 = bx % tiles_of_rows, piece = bx / tiles_of_rows;
-    const int rows = a.count * a.group;
     const int row = tile0 * kSpanRows + col;
     const int last_row = min(rows, (tile0 + 1) * kSpanRows) - 1;
     const bool live = row < rows;
@@ -44,7 +55,7 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
     // New tokens (at most one row tile, so at most 16): token wave + NW i's rows, ahead of everything that waits for the
     // unit's position or length.
     NewRow fresh[kSpanRows / NW];
-    if (a.new_k) {
+    if (!PAGED && a.new_k) {
 #pragma unroll
         for (int i = 0; i < kSpanRows / NW; ++i) {
             if (wave + NW * i >= a.count) break;
@@ -64,18 +75,33 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
         full_low = p1 >= a.window ? p1 - a.window : -1;
         full_high = p0;
         alone = p0 == p1;
+    } else if constexpr (PAGED) {
+        const int p0 = req.first + tile0 * kSpanRows / a.group, p1 = req.first + last_row / a.group;
+        runs = page_runs(req.first < 0 ? -1 : p0, p1, a.window, kSpanTile);
+        own = req.first + (live ? row : last_row) / a.group;
+        full_low = a.window > 0 && p1 >= a.window ? p1 - a.window : -1;
+        full_high = p0;
+        alone = p0 == p1 && full_low < runs.begin1;
     } else {
         const int n = min(a.lengths ? a.lengths[unit] : a.length, a.length);
         runs.n0 = runs.pinned = n > 0 ? n : 0;
     }
     const int tiles0 = span_tiles(runs.n0), tiles = tiles0 + span_tiles(runs.n1);
-    const int begin = piece * a.per, end = min(begin + a.per, tiles);
+    int per = a.per, pieces = a.splits;
+    if constexpr (PAGED) {
+        per = max(a.per, ((tiles + a.splits - 1) / a.splits + NW - 1) / NW * NW);
+        pieces = (tiles + per - 1) / per;
+        if (piece > 0 && piece >= pieces) return;
+    }
+    const int begin = piece * per, end = min(begin + per, tiles);
 
     const size_t row0 = (static_cast<size_t>(unit) * a.kvheads + kh) * cap;
     const auto rk = buffer_rsrc(a.c.k8 + row0 * HD, static_cast<uint32_t>(cap) * HD);
     const auto rv = buffer_rsrc(a.c.v8 + row0 * HD, static_cast<uint32_t>(cap) * HD);
     const auto rks = buffer_rsrc(a.c.ks + row0, static_cast<uint32_t>(cap) * 4u);
     const auto rvs = buffer_rsrc(a.c.vs + row0, static_cast<uint32_t>(cap) * 4u);
+    PageReader<HD> pages;
+    if constexpr (PAGED) pages = PageReader<HD>(a, unit, kh);
 
     // first slot of a tile, and the first slot behind its run
     auto slot0 = [&](int tile) { return tile < tiles0 ? tile * kSpanTile : runs.begin1 + (tile - tiles0) * kSpanTile; };
@@ -85,21 +111,38 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
         uint32_t k[4][kSteps][2];
         uint32_t v[4][4][(VB + 3) / 4];
         float ks, vs;
+        uint32_t live;  // paged: of each 16 positions, whether the request has their page
+    };
+    // Pages of a tile's pieces of 16 positions, loaded a tile ahead of them.
+    struct Ids {
+        int id[4];
+    };
+    auto find = [&](Ids &ids, int tile) {
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ids.id[i] = pages.id(slot0(tile) + 16 * i);
+        }
     };
     // Loads past the cache's rows read zero; slots of a tile behind its run are masked in compute.
-    auto load = [&](Tile &T, int tile) {
-        const uint32_t s0 = static_cast<uint32_t>(slot0(tile));
+    auto load = [&](Tile &T, int tile, const Ids &ids) {
+        const uint32_t s0 = PAGED ? 0u : static_cast<uint32_t>(slot0(tile));
         const uint32_t kb = (s0 + col) * HD + quad * kBytes;
+        auto rk_of = [&](int i) {
+            if constexpr (PAGED) return pages.k_codes(ids.id[i], slot0(tile) + 16 * i);
+            else return rk;
+        };
+        constexpr uint32_t step = PAGED ? 0 : 16 * HD;  // paged: every 16 rows have a base of their own
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+            const auto rk = rk_of(i);
             if constexpr (HD == 32) {
-                const auto w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rk, kb + i * 16 * HD, 0, 0));
+                const auto w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rk, kb + i * step, 0, 0));
                 T.k[i][0][0] = w.x;
                 T.k[i][0][1] = w.y;
             } else {
 #pragma unroll
                 for (int h = 0; h < kSteps / 2; ++h) {
-                    const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(rk, kb + i * 16 * HD + h * 16, 0, 0);
+                    const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(rk, kb + i * step + h * 16, 0, 0);
                     T.k[i][2 * h][0] = w.x;
                     T.k[i][2 * h][1] = w.y;
                     T.k[i][2 * h + 1][0] = w.z;
@@ -107,14 +150,32 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
                 }
             }
         }
-        T.ks = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rks, (s0 + lane) * 4u, 0, 0));
-        T.vs = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rvs, (s0 + lane) * 4u, 0, 0));
-        const uint32_t vb = (s0 + 4 * quad) * HD + col * VB;
+        if constexpr (PAGED) {
+            T.live = 0;
+            const float *scales = nullptr;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) {
+                T.live |= ids.id[i] >= 0 ? 1u << i : 0u;
+                const float *of = pages.k_scales(ids.id[i], slot0(tile) + 16 * i);
+                scales = i == 0 || quad == i ? of : scales;
+            }
+            T.ks = scales[col];
+            T.vs = scales[col + (1 << pages.shift)];
+        } else {
+            T.ks = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rks, (s0 + lane) * 4u, 0, 0));
+            T.vs = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rvs, (s0 + lane) * 4u, 0, 0));
+        }
+        const uint32_t vb = (s0 + 4 * quad) * HD + col * VB;
+        auto rv_of = [&](int i) {
+            if constexpr (PAGED) return pages.v_codes(ids.id[i], slot0(tile) + 16 * i);
+            else return rv;
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const auto rv = rv_of(i);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const uint32_t at = vb + (16 * i + u) * HD;
+                const uint32_t at = vb + i * step + u * HD;
                 if constexpr (VB == 8) {
                     const auto w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, at, 0, 0));
                     T.v[i][u][0] = w.x;
@@ -125,6 +186,7 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
                     T.v[i][u][0] = static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(rv, at, 0, 0));
                 }
             }
+        }
     };
 
     // A new token's slot; -1: not in this block's tiles. Its tile in `in`.
@@ -138,19 +200,26 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
     // The first tile is on its way before the new tokens are stored, unless it holds one of them; the next tile is loaded
     // before a tile is computed.
     Tile cur, nxt;
+    Ids ids;
     int tile = begin + wave;
+    find(ids, tile);
     bool wait = false;
-    if (a.new_k) {
+    if (!PAGED && a.new_k) {
         for (int i = 0; i < a.count; ++i) {
             int in = -1;
             wait = wait || (new_slot(i, in) >= 0 && in == tile);
         }
     }
-    if (!wait) load(cur, tile);
+    if (!wait) load(cur, tile, ids);
+    find(ids, tile + NW);
 
     // q as operand B: lane (row col, quad) holds dimensions quad * HD / 4 .. in steps of eight
-    const size_t orow = (static_cast<size_t>(unit) * a.count + (live ? row : 0) / a.group) * a.heads + kh * a.group +
-                        (live ? row : 0) % a.group;
+    auto out_row = [&](int r) {
+        size_t token = static_cast<size_t>(unit) * a.count;
+        if constexpr (PAGED) token = req.token;
+        return (token + r / a.group) * a.heads + kh * a.group + r % a.group;
+    };
+    const size_t orow = out_row(live ? row : 0);
     Terms q[kSteps];
     {
         float x[kSteps][8];
@@ -166,7 +235,7 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
         for (int c = 0; c < kSteps; ++c) q[c] = split8(x[c]);
     }
 
-    if (a.new_k) {
+    if (!PAGED && a.new_k) {
 #pragma unroll
         for (int i = 0; i < kSpanRows / NW; ++i) {
             if (wave + NW * i >= a.count) break;
@@ -176,7 +245,7 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
         }
         __syncthreads();  // (and the block's stores before its loads of those rows)
     }
-    if (wait) load(cur, tile);
+    if (wait) load(cur, tile, ids);
 
     float m = -INFINITY, l = 0.0f;
     f32x4 acc[VB];
@@ -222,16 +291,17 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
             masked |= !alone && (all_pinned ? s0 + kSpanTile - 1 > full_high
                                             : s0 < runs.pinned || s0 + shift <= full_low || s0 + kSpanTile - 1 + shift > full_high);
         }
+        if constexpr (PAGED) masked |= T.live != 15u || (!alone && (s0 <= full_low || s0 + kSpanTile - 1 > full_high));
         if (masked) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const bool ok = s0 + 16 * i + 4 * quad + u < behind;
+                    const bool ok = s0 + 16 * i + 4 * quad + u < behind && (!PAGED || (T.live >> i & 1u));
                     x[i][u] = ok ? x[i][u] : -INFINITY;
                     vs[i][u] = ok ? vs[i][u] : 0.0f;
                 }
-            if (RING && !alone) {
+            if ((RING || PAGED) && !alone) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -239,13 +309,13 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
                         const int slot = s0 + 16 * i + 4 * quad + u;
                         const bool pin = tile < tiles0 && slot < runs.pinned;
                         const int p = pin ? slot : slot + (tile < tiles0 ? runs.shift0 : runs.shift1);
-                        const bool ok = p <= own && (pin || own - p < a.window);
+                        const bool ok = p <= own && (pin || (PAGED && a.window == 0) || own - p < a.window);
                         x[i][u] = ok ? x[i][u] : -INFINITY;
                         vs[i][u] = ok ? vs[i][u] : 0.0f;
                     }
             }
         }
-        if (a.scores && live) {
+        if (!PAGED && a.scores && live) {
             float *to = a.scores + (static_cast<size_t>(unit) * a.kvheads * a.group + kh * a.group + row) * a.score_stride + s0;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -302,7 +372,8 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
     };
 
     for (; tile < end; tile += NW) {
-        load(nxt, tile + NW);
+        load(nxt, tile + NW, ids);
+        find(ids, tile + 2 * NW);
         asm volatile("" ::: "memory");
         compute(cur, tile);
         cur = nxt;
@@ -311,6 +382,11 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
     // the waves' results over their own maxima
     l += butterfly_partner<16>(l, lane);
     l += butterfly_partner<32>(l, lane);
+    bool finish = !a.rec_o;
+    if constexpr (PAGED) {
+        finish = pieces <= 1;
+        if (!finish && piece == 0 && wave == 0 && quad == 0 && live) a.records[orow] = pieces;
+    }
     if (quad == 0) {
         sm[wave][col] = m;
         sl[wave][col] = l;
@@ -342,8 +418,8 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
             o[2] = __builtin_fmaf(f, p.z, o[2]);
             o[3] = __builtin_fmaf(f, p.w, o[3]);
         }
-        const size_t at = (static_cast<size_t>(unit) * a.count + grow / a.group) * a.heads + kh * a.group + grow % a.group;
-        if (!a.rec_o) {
+        const size_t at = out_row(grow);
+        if (finish) {
             const float inv = L > 0 ? 1.0f / L : 0.0f;
             *reinterpret_cast<float4 *>(a.out + at * HD + d) =
                 L > 0 ? make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv) : make_float4(0, 0, 0, 0);
@@ -357,10 +433,10 @@ __device__ __forceinline__ void span_rows(const SpanArgs &a, int bx, int kh, int
 
 // Block `b` of a launch of all units, kv heads, row tiles and pieces. The pieces are slowest: those behind the end of a
 // short sequence come last, and the others spread over the compute units.
-template <int HD, int NW, bool RING>
-__device__ __forceinline__ void span_block(const SpanArgs &a, int b) {
+template <int HD, int NW, Keys K, class A>
+__device__ __forceinline__ void span_block(const A &a, int b) {
     const int rest = b / a.kvheads;
-    span_rows<HD, NW, RING>(a, rest / a.units, b % a.kvheads, rest % a.units);
+    span_rows<HD, NW, K>(a, rest / a.units, b % a.kvheads, rest % a.units);
 }
 
 }  // namespace

@@ -571,7 +571,7 @@ __global__ __launch_bounds__(256, 2) void span_wide_kernel(SpanArgs a) {
 template <int HD>
 __global__ __launch_bounds__(256, 2) void span_wide_own_kernel(SpanArgs far, SpanArgs own, int far_blocks) {
     if (static_cast<int>(blockIdx.x) < far_blocks) span_wide<HD, false>(far, blockIdx.x);
-    else span_block<HD, 4, false>(own, blockIdx.x - far_blocks);
+    else span_block<HD, 4, Keys::Flat>(own, blockIdx.x - far_blocks);
 }
 
 int64_t wide_blocks(const SpanArgs &a) {

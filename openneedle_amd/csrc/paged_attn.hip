@@ -2,7 +2,7 @@
 // mathematics, the operands and the records are span_kernels.hip's; a tile's pages are looked up ahead of its loads.
 #include "paged.h"
 #include "span_join.h"
-#include "span_rows.h"
+#include "span_wide.h"
 
 namespace nd {
 
@@ -11,6 +11,13 @@ namespace {
 template <int HD, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void paged_kernel(PagedSpanArgs a) {
     span_block<HD, NW, Keys::Paged>(a, blockIdx.x);
+}
+
+// The blocks of 128 rows first: they take the longest.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void paged_wide_kernel(PagedSpanArgs a, int blocks) {
+    if (static_cast<int>(blockIdx.x) < blocks) span_wide<HD, Keys::Paged>(a, blockIdx.x);
+    else span_block<HD, 4, Keys::Paged>(a, blockIdx.x - blocks);
 }
 
 template <int HD, int G>
@@ -22,7 +29,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedSpanArgs a, int64_
 
 template <int HD>
 void launch_hd(const PagedSpanArgs &a, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.splits) * a.row_tiles * a.kvheads * a.units));
+    const int64_t wide = static_cast<int64_t>(a.wide_blocks) * a.wide_splits * a.kvheads;
+    const dim3 grid(static_cast<unsigned>(wide + static_cast<int64_t>(a.splits) * a.row_tiles * a.kvheads * a.units));
+    if (wide > 0) {
+        hipLaunchKernelGGL((paged_wide_kernel<HD>), grid, dim3(256), 0, s, a, static_cast<int>(wide));
+        ND_HIP(hipGetLastError());
+        return;
+    }
     if (a.waves == 4) hipLaunchKernelGGL((paged_kernel<HD, 4>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((paged_kernel<HD, 8>), grid, dim3(512), 0, s, a);
     ND_HIP(hipGetLastError());

@@ -21,6 +21,25 @@ __device__ __forceinline__ Request request(const PagedSpanArgs &a, int r) {
     return q;
 }
 
+// Block b of 128 rows: request r has those from starts[r] * group / 128 + r on, at least as many as it has row tiles (of two
+// requests' whole and cut tiles, one more than the rows before them fill). 64 of the requests are looked at at a time.
+struct WideBlock {
+    int unit, row;
+};
+__device__ __forceinline__ WideBlock wide_block(const PagedSpanArgs &a, int b, int lane) {
+    auto from = [&](int r) { return max(0, min(a.starts[r], a.tokens)) * a.group / kWideRows + r; };
+    int low = 0, n = a.units;
+    while (n > 1) {
+        const int step = (n + 63) / 64, i = lane * step;
+        const bool before = i == 0 || (i < n && from(low + i) <= b);
+        const int at = (__popcll(__ballot(before)) - 1) * step;
+        low += at;
+        n = min(step, n - at);
+    }
+    low = __builtin_amdgcn_readfirstlane(low);
+    return WideBlock{low, max(0, b - __builtin_amdgcn_readfirstlane(from(low))) * kWideRows};
+}
+
 // The pages of a request and kv head. A page outside the cache is none (-1): its rows read as zeros and are masked.
 template <int HD>
 struct PageReader {

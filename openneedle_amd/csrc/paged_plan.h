@@ -6,6 +6,8 @@
 
 namespace nd {
 
+constexpr int kPagedSmall = 64;
+
 // Requests of at most `small` rows (tokens times query heads per kv head) are in `row_tiles` blocks of 16 rows each, others
 // in blocks of 128 (`wide_blocks` of them at most).
 struct PagedCut {
@@ -18,9 +20,28 @@ inline PagedCut cut_paged(int cus, int head_dim, int requests, int tokens, int c
     PagedCut c;
     const int64_t rows = int64_t(count) * group;
     const int keys = window > 0 ? static_cast<int>(std::min<int64_t>(length, int64_t(window) + count - 1)) : length;
-    c.small = 1 << 30;
-    c.row_tiles = static_cast<int>((rows + kSpanRows - 1) / kSpanRows);
-    c.rows = cut_span(cus, head_dim, rows, int64_t(requests) * kvheads, keys, keys, 2, false, false);
+    // Up to 64 rows, blocks of 16 turn a request's keys over faster than one block of 128 with few rows in it.
+    c.small = kPagedSmall;
+    if (rows <= c.small) {
+        c.row_tiles = static_cast<int>((rows + kSpanRows - 1) / kSpanRows);
+        c.rows = cut_span(cus, head_dim, rows, int64_t(requests) * kvheads, keys, keys, 2, false, false);
+        return c;
+    }
+    static const SpanRate kFour[3] = {{4, 4, 5, 1.2, 1.6}, {4, 4, 5, 1.25, 2.4}, {4, 4, 5, 1.85, 4.1}};
+    static const SpanRate kWide[3] = {{4, 1, 6, 1.15, 1.5}, {4, 1, 6, 1.15, 1.7}, {4, 1, 6, 1.2, 2.3}};
+    const int h = head_dim == 32 ? 0 : head_dim == 64 ? 1 : 2;
+    const double row = 2.0 * (head_dim + 4);
+    // every request has one, but only those with tokens and room for more of them have more
+    c.wide_blocks = static_cast<int>(int64_t(tokens) * group / kWideRows) + requests;
+    const int64_t filled = std::max<int64_t>(1, int64_t(tokens) * group / kWideRows);
+    const double record = double(tokens) * group * kvheads * head_dim * 8 / 3e6;
+    best_cut(c.wide, cus, filled * kvheads, std::max(1, wide_tiles(keys)), keys * row, kWide[h], record, 3.5);
+    if (requests == 1) {  // (whatever its tokens turn out to be)
+        c.small = 0;
+        return c;
+    }
+    c.row_tiles = (c.small + kSpanRows - 1) / kSpanRows;
+    best_cut(c.rows, cus, int64_t(requests) * kvheads, std::max(1, span_tiles(keys)), keys * row, kFour[h], 0.5, 3.5);
     return c;
 }
 

@@ -15,6 +15,8 @@ inline const char *check_pages(int layers, int pages, int page_size, int kvheads
         return "paged cache: page_size must be 16, 32, 64, 128 or 256";
     if (head_dim != 32 && head_dim != 64 && head_dim != 128) return "paged cache: head_dim must be 32, 64 or 128";
     if (kvheads > kMaxGrid) return "paged cache: at most 65535 kv heads";
+    if (int64_t(kvheads) * page_size * (2 * head_dim + 8) >= (int64_t(1) << 31))
+        return "paged cache: the kv heads' rows of a page must be below 2^31 bytes";
     if (int64_t(pages) * page_size >= (int64_t(1) << 31)) return "paged cache: pages * page_size must be below 2^31";
     return nullptr;
 }

@@ -8,6 +8,16 @@ namespace nd {
 // Memory that no kernel of the running launch writes, read through the scalar cache where the address is uniform.
 #define ND_CONST __attribute__((address_space(4)))
 
+// The kernel's arguments, as the first of which it has `a`, read again where this is called instead of held in registers.
+template <class A>
+__device__ __forceinline__ const ND_CONST A &late(const PagedSpanArgs &) {
+    auto p = (const ND_CONST A *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *p;
+}
+template <class A>
+__device__ __forceinline__ const A &late(const SpanArgs &a) { return a; }
+
 // A request's tokens: the first one's row of q and its position, and how many. A request that does not lie in its table (or
 // at a negative position) attends nothing.
 struct Request {
@@ -45,20 +55,24 @@ template <int HD>
 struct PageReader {
     const ND_CONST int *table;
     const uint8_t *at;
-    size_t page_bytes;  // of all kv heads
+    uint32_t page_bytes;  // of all kv heads
     int width, pages, shift;
     __device__ __forceinline__ PageReader() = default;
     __device__ __forceinline__ PageReader(const PagedSpanArgs &a, int unit, int kh)
         : table((const ND_CONST int *)(a.tables + static_cast<size_t>(unit) * a.width)),
           at(a.pool.at + static_cast<size_t>(kh) * page_block_bytes(a.pool.shift, HD)),
-          page_bytes(static_cast<size_t>(a.pool.kvheads) * page_block_bytes(a.pool.shift, HD)), width(a.width),
+          page_bytes(a.pool.kvheads * page_block_bytes(a.pool.shift, HD)), width(a.width),
           pages(a.pool.pages), shift(a.pool.shift) {}
-    __device__ __forceinline__ int id(int position) const {
-        const int i = position >> shift;
-        const int p = table[min(i, width - 1)];
-        return i < width && static_cast<unsigned>(p) < static_cast<unsigned>(pages) ? p : -1;
+    // The table's entry for a position (the same for all lanes, or of every lane's own), loaded ahead of its use, and the
+    // page that it says.
+    __device__ __forceinline__ int entry(int position) const { return table[min(position >> shift, width - 1)]; }
+    __device__ __forceinline__ int entry_of_lane(int position) const {
+        return ((const ND_GLOBAL int *)(uintptr_t)table)[min(position >> shift, width - 1)];
     }
-    __device__ __forceinline__ const uint8_t *block(int id) const { return at + max(id, 0) * page_bytes; }
+    __device__ __forceinline__ int page(int entry, int position) const {
+        return position >> shift < width && static_cast<unsigned>(entry) < static_cast<unsigned>(pages) ? entry : -1;
+    }
+    __device__ __forceinline__ const uint8_t *block(int id) const { return at + static_cast<uint64_t>(static_cast<uint32_t>(max(id, 0))) * page_bytes; }
     __device__ __forceinline__ int off(int position) const { return position & ((1 << shift) - 1); }
     // 16 rows from a position on (a multiple of 16); past them, and of no page, zeros
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t k_codes(int id, int position) const {

@@ -102,7 +102,6 @@ __device__ __forceinline__ void span_rows(const A &a, int bx, int kh, int unit) 
     const auto rvs = buffer_rsrc(a.c.vs + row0, static_cast<uint32_t>(cap) * 4u);
     PageReader<HD> pages;
     if constexpr (PAGED) pages = PageReader<HD>(a, unit, kh);
-
     // first slot of a tile, and the first slot behind its run
     auto slot0 = [&](int tile) { return tile < tiles0 ? tile * kSpanTile : runs.begin1 + (tile - tiles0) * kSpanTile; };
     auto stop = [&](int tile) { return tile < tiles0 ? runs.n0 : runs.begin1 + runs.n1; };
@@ -113,22 +112,25 @@ __device__ __forceinline__ void span_rows(const A &a, int bx, int kh, int unit) 
         float ks, vs;
         uint32_t live;  // paged: of each 16 positions, whether the request has their page
     };
-    // Pages of a tile's pieces of 16 positions, loaded a tile ahead of them.
-    struct Ids {
+    // Pages of a tile's pieces of 16 positions, looked up a tile ahead of them.
+    struct Pages {
         int id[4];
     };
-    auto find = [&](Ids &ids, int tile) {
+    auto find = [&](Pages &of, int tile) {
         if constexpr (PAGED) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ids.id[i] = pages.id(slot0(tile) + 16 * i);
+            for (int i = 0; i < 4; ++i) {
+                const int p = slot0(tile) + 16 * i;
+                of.id[i] = pages.page(pages.entry(p), p);
+            }
         }
     };
     // Loads past the cache's rows read zero; slots of a tile behind its run are masked in compute.
-    auto load = [&](Tile &T, int tile, const Ids &ids) {
+    auto load = [&](Tile &T, int tile, const Pages &of) {
         const uint32_t s0 = PAGED ? 0u : static_cast<uint32_t>(slot0(tile));
         const uint32_t kb = (s0 + col) * HD + quad * kBytes;
         auto rk_of = [&](int i) {
-            if constexpr (PAGED) return pages.k_codes(ids.id[i], slot0(tile) + 16 * i);
+            if constexpr (PAGED) return pages.k_codes(of.id[i], slot0(tile) + 16 * i);
             else return rk;
         };
         constexpr uint32_t step = PAGED ? 0 : 16 * HD;  // paged: every 16 rows have a base of their own
@@ -155,9 +157,9 @@ __device__ __forceinline__ void span_rows(const A &a, int bx, int kh, int unit) 
             const float *scales = nullptr;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                T.live |= ids.id[i] >= 0 ? 1u << i : 0u;
-                const float *of = pages.k_scales(ids.id[i], slot0(tile) + 16 * i);
-                scales = i == 0 || quad == i ? of : scales;
+                T.live |= of.id[i] >= 0 ? 1u << i : 0u;
+                const float *at = pages.k_scales(of.id[i], slot0(tile) + 16 * i);
+                scales = i == 0 || quad == i ? at : scales;
             }
             T.ks = scales[col];
             T.vs = scales[col + (1 << pages.shift)];
@@ -167,7 +169,7 @@ __device__ __forceinline__ void span_rows(const A &a, int bx, int kh, int unit) 
         }
         const uint32_t vb = (s0 + 4 * quad) * HD + col * VB;
         auto rv_of = [&](int i) {
-            if constexpr (PAGED) return pages.v_codes(ids.id[i], slot0(tile) + 16 * i);
+            if constexpr (PAGED) return pages.v_codes(of.id[i], slot0(tile) + 16 * i);
             else return rv;
         };
 #pragma unroll
@@ -200,9 +202,9 @@ __device__ __forceinline__ void span_rows(const A &a, int bx, int kh, int unit) 
     // The first tile is on its way before the new tokens are stored, unless it holds one of them; the next tile is loaded
     // before a tile is computed.
     Tile cur, nxt;
-    Ids ids;
+    Pages of;
     int tile = begin + wave;
-    find(ids, tile);
+    find(of, tile);
     bool wait = false;
     if (!PAGED && a.new_k) {
         for (int i = 0; i < a.count; ++i) {
@@ -210,8 +212,8 @@ __device__ __forceinline__ void span_rows(const A &a, int bx, int kh, int unit) 
             wait = wait || (new_slot(i, in) >= 0 && in == tile);
         }
     }
-    if (!wait) load(cur, tile, ids);
-    find(ids, tile + NW);
+    if (!wait) load(cur, tile, of);
+    find(of, tile + NW);
 
     // q as operand B: lane (row col, quad) holds dimensions quad * HD / 4 .. in steps of eight
     auto out_row = [&](int r) {
@@ -245,7 +247,7 @@ __device__ __forceinline__ void span_rows(const A &a, int bx, int kh, int unit) 
         }
         __syncthreads();  // (and the block's stores before its loads of those rows)
     }
-    if (wait) load(cur, tile, ids);
+    if (wait) load(cur, tile, of);
 
     float m = -INFINITY, l = 0.0f;
     f32x4 acc[VB];
@@ -372,8 +374,8 @@ __device__ __forceinline__ void span_rows(const A &a, int bx, int kh, int unit) 
     };
 
     for (; tile < end; tile += NW) {
-        load(nxt, tile + NW, ids);
-        find(ids, tile + 2 * NW);
+        load(nxt, tile + NW, of);
+        find(of, tile + 2 * NW);
         asm volatile("" ::: "memory");
         compute(cur, tile);
         cur = nxt;

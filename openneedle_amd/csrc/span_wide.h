@@ -130,9 +130,9 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
     __shared__ u32x4 vf[2][2][DT][kFrag];
     __shared__ __attribute__((aligned(16))) float sc[4][2][kWideTile];  // K (times scale) and V scales, by tile modulo 4
     // of the tile's slots in its run: the exponent of the largest finite V scale, plus kOddTile where one is infinite or
-    // NaN; and the largest |K scale|
+    // NaN (paged: in the lower half, and in the upper one, of each 16 positions, whether the request has their page); and
+    // the largest |K scale|
     __shared__ int2 about[4];
-    __shared__ uint32_t paged[PAGED ? 4 : 1];  // of each 16 of the tile's positions, whether the request has their page
 
     const int t = threadIdx.x, lane = t & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -191,8 +191,10 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
         if (piece > 0 && piece >= pieces) return;
     }
     const int begin = piece * per, end = min(begin + per, tiles);
-    auto slot0 = [&](int tile) { return tile < tiles0 ? tile * kWideTile : runs.begin1 + (tile - tiles0) * kWideTile; };
-    auto stop = [&](int tile) { return tile < tiles0 ? runs.n0 : runs.begin1 + runs.n1; };
+    auto slot0 = [&](int tile) {
+        return !PAGED && tile < tiles0 ? tile * kWideTile : runs.begin1 + (tile - (PAGED ? 0 : tiles0)) * kWideTile;
+    };
+    auto stop = [&](int tile) { return !PAGED && tile < tiles0 ? runs.n0 : runs.begin1 + runs.n1; };
 
     const size_t row0 = (static_cast<size_t>(unit) * a.kvheads + kh) * cap;
     const auto rk = buffer_rsrc(a.c.k8 + row0 * HD, static_cast<uint32_t>(cap) * HD);
@@ -216,38 +218,44 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
     struct RawV {
         uint32_t v[4];
     };
-    // Pages of the two pieces of 16 positions of K's next tile and, one tile behind, of V's; looked up a tile ahead.
-    int k_page[2] = {-1, -1}, v_page[2] = {-1, -1};
+    // A wave brings rows of one half of a tile (of rows of 32 values those of both, the second's on lanes 32 .. 63). Where
+    // they begin, of K's last tile and of V's, one tile behind; and the table's entries for the positions of K's next
+    // one, loaded a tile ahead (as vectors: scalar loads under way would be waited for with every LDS operation).
+    constexpr int kHalves = HD == 32 ? 2 : 1;
+    const int part = HD == 32 ? 0 : kBoth ? wave >> 1 : wave & 1;
+    const uint8_t *k_at[kHalves] = {}, *v_at[kHalves] = {};
+    int entry = -1;
     auto find = [&](int tile) {
+        if constexpr (PAGED) entry = pages.entry_of_lane(slot0(tile) + col);
+    };
+    // what find has found for K's next tile (in the loop ahead of the products, whose issue it does not delay)
+    auto locate = [&](int tile) {
         if constexpr (PAGED) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                v_page[i] = k_page[i];
-                k_page[i] = pages.id(slot0(tile) + 16 * i);
+            for (int i = 0; i < kHalves; ++i) {
+                const int p = slot0(tile) + 16 * (part + i);
+                v_at[i] = k_at[i];
+                k_at[i] = pages.block(pages.page(__builtin_amdgcn_readlane(entry, 16 * (part + i)), p)) + pages.off(p) * HD;
             }
         }
     };
-    // A wave's rows are in one of the pieces, but for rows of 32, which it has of both: then lanes 32 .. 63 the second's.
-    const int k_piece = kBoth ? wave >> 1 : wave & 1, v_piece = kBoth ? wave >> 1 : (wave - kRoleWaves) & 1;
     auto fetch_k = [&](RawK &r, int tile) {
         if constexpr (PAGED) {
             const uint32_t at = k_role ? kc * 16 % (16 * HD) : kNone;
             if constexpr (HD == 32) {
-                const u32x4 a0 = __builtin_amdgcn_raw_buffer_load_b128(pages.k_codes(k_page[0], slot0(tile)), half ? kNone : at, 0, 0);
-                const u32x4 a1 = __builtin_amdgcn_raw_buffer_load_b128(pages.k_codes(k_page[1], slot0(tile) + 16),
-                                                                       half ? at : kNone, 0, 0);
-                r.k = a0 | a1;
+                if (k_role) r.k = *(const ND_GLOBAL u32x4 *)((half ? k_at[1] : k_at[0]) + at);
             } else {
-                r.k = __builtin_amdgcn_raw_buffer_load_b128(
-                    pages.k_codes(k_piece ? k_page[1] : k_page[0], slot0(tile) + 16 * k_piece), at, 0, 0);
+                r.k = __builtin_amdgcn_raw_buffer_load_b128(buffer_rsrc(k_at[0], 16 * HD), at, 0, 0);
             }
             r.s[0] = r.s[1] = 0.0f;
-            r.paged = (k_page[0] >= 0 ? 1u : 0u) | (k_page[1] >= 0 ? 2u : 0u);
+            r.paged = 0;
             if (wave == kScaleWave) {
-                const float *first = pages.k_scales(k_page[0], slot0(tile)), *second = pages.k_scales(k_page[1], slot0(tile) + 16);
-                const float *of = (col < 16 ? first : second) + (col & 15);
+                const int scale_page = pages.page(entry, slot0(tile) + col);
+                const float *of = pages.k_scales(scale_page, slot0(tile) + col);
                 r.s[0] = of[0];
                 r.s[1] = of[1 << pages.shift];
+                const uint64_t has = __ballot(scale_page >= 0);
+                r.paged = (has & 1u) | (has >> 15 & 2u);
             }
             return;
         }
@@ -261,15 +269,15 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
         if constexpr (PAGED) {
             const uint32_t at = v_role ? 4 * v_keys % 16 * HD + v_dims * 4 : kNone;
             if constexpr (HD == 32) {
-                const auto first = pages.v_codes(v_page[0], slot0(tile)), second = pages.v_codes(v_page[1], slot0(tile) + 16);
+                if (v_role) {
+                    const auto row = (const ND_GLOBAL uint32_t *)((half ? v_at[1] : v_at[0]) + (HD << pages.shift) + at);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    r.v[j] = __builtin_amdgcn_raw_buffer_load_b32(first, half ? kNone : at + j * HD, 0, 0) |
-                             __builtin_amdgcn_raw_buffer_load_b32(second, half ? at + j * HD : kNone, 0, 0);
+                    for (int j = 0; j < 4; ++j) r.v[j] = row[j * HD / 4];
+                }
             } else {
-                const auto rv = pages.v_codes(v_piece ? v_page[1] : v_page[0], slot0(tile) + 16 * v_piece);
+                const auto rows = buffer_rsrc(v_at[0] + (HD << pages.shift), 16 * HD);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) r.v[j] = __builtin_amdgcn_raw_buffer_load_b32(rv, at + j * HD, 0, 0);
+                for (int j = 0; j < 4; ++j) r.v[j] = __builtin_amdgcn_raw_buffer_load_b32(rows, at + j * HD, 0, 0);
             }
             return;
         }
@@ -287,10 +295,7 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
         }
         if (wave == kScaleWave) {
             bool in = slot0(tile) + col < stop(tile);
-            if constexpr (PAGED) {
-                in = in && (r.paged >> (col >> 4) & 1u);
-                if (lane == 0) paged[sb] = r.paged;
-            }
+            if constexpr (PAGED) in = in && (r.paged >> (col >> 4) & 1u);
             const float ks = in ? r.s[0] * a.scale : 0.0f;
             float vs = in ? r.s[1] : 0.0f;
             // A V row of zeros, whose scale the quantiser makes 1, adds nothing: scale 0, so that neither M nor a row's
@@ -298,15 +303,11 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
             if (__builtin_expect(__any(vs == 1.0f), 0)) {
                 uint32_t codes = 0;  // of a half of the row
                 if constexpr (PAGED) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int p = slot0(tile) + 16 * i;
-                        const auto rv = pages.v_codes(pages.id(p), p);
-#pragma unroll
-                        for (int c = 0; c < HD / 2; c += 4)
-                            codes |= __builtin_amdgcn_raw_buffer_load_b32(
-                                rv, col >> 4 == i ? (col & 15) * HD + half * (HD / 2) + c : kNone, 0, 0);
-                    }
+                    const int p = slot0(tile) + col;
+                    const uint32_t *row = reinterpret_cast<const uint32_t *>(pages.block(pages.page(pages.entry_of_lane(p), p)) + (HD << pages.shift) +
+                                                                             pages.off(p) * HD + half * (HD / 2));
+#pragma unroll 1
+                    for (int c = 0; c < HD / 8; ++c) codes |= row[c];
                 }
 #pragma unroll
                 for (int c = 0; !PAGED && c < HD / 2; c += 4)
@@ -321,7 +322,8 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
             const float most = group_max<32>(half ? odd ? 0.0f : v : fabsf(ks), lane);
             const float v_most = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, most), 32));
             const int ve = (v_most > 0 ? __builtin_amdgcn_frexp_expf(v_most) : 0) + (__any(odd) ? kOddTile : 0);
-            if (lane == 0) about[sb] = make_int2(ve, __builtin_bit_cast(int, most));
+            const int code = PAGED ? (ve & 0xFFFF) | static_cast<int>(r.paged << 16) : ve;
+            if (lane == 0) about[sb] = make_int2(code, __builtin_bit_cast(int, most));
         }
     };
     auto place_v = [&](const RawV &r, int tile) {
@@ -342,8 +344,10 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
     RawK rk_next, rk_first;
     RawV rv_next;
     find(begin);
+    locate(begin);
     fetch_k(rk_first, begin);
     find(begin + 1);
+    locate(begin + 1);
     fetch_k(rk_next, begin + 1);
     fetch_v(rv_next, begin);
     find(begin + 2);
@@ -351,6 +355,7 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
         place_k(rk_first, begin);
         place_k(rk_next, begin + 1);
         place_v(rv_next, begin);
+        locate(begin + 2);
         fetch_k(rk_next, begin + 2);
         fetch_v(rv_next, begin + 1);
         find(begin + 3);
@@ -359,6 +364,7 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
         for (int tile = begin; tile < end; ++tile) {
             place_v(rv_next, tile + 1);
             place_k(rk_next, tile + 2);
+            locate(tile + 3);
             fetch_k(rk_next, tile + 3);
             fetch_v(rv_next, tile + 2);
             find(tile + 4);
@@ -498,6 +504,7 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
     place_k(rk_first, begin);
     place_k(rk_next, begin + 1);
     place_v(rv_next, begin);
+    locate(begin + 2);
     fetch_k(rk_next, begin + 2);
     fetch_v(rv_next, begin + 1);
     find(begin + 3);
@@ -507,8 +514,11 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
     __syncthreads();  // every wave has its first scores before K's buffer is written again
     for (int tile = begin; tile < end; ++tile) {
         const int vb = (tile - begin) & 1, sb = (tile - begin) & 3;
-        const int s0 = slot0(tile), behind = stop(tile);
-        const int code = __builtin_amdgcn_readfirstlane(about[sb].x);
+        int s0 = slot0(tile);
+        const int behind = stop(tile);
+        if constexpr (PAGED) asm volatile("" : "+s"(s0));  // (what follows of it is not kept in registers across tiles)
+        const int word = __builtin_amdgcn_readfirstlane(about[sb].x);
+        const int code = PAGED ? static_cast<int16_t>(word & 0xFFFF) : word;
         const int ve = code > kOddTile / 2 ? code - kOddTile : code;
         f32x16 x;
 #pragma unroll
@@ -526,9 +536,8 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
             masked |= all_pinned ? s0 + kWideTile - 1 > full_high
                                  : s0 < runs.pinned || s0 + shift <= full_low || s0 + kWideTile - 1 + shift > full_high;
         }
-        uint32_t has = 3u;
+        const uint32_t has = static_cast<uint32_t>(word) >> 16;
         if constexpr (PAGED) {
-            has = __builtin_amdgcn_readfirstlane(paged[sb]);
             masked |= has != 3u || s0 <= full_low || s0 + kWideTile - 1 > full_high;
         }
         uint32_t gone = 0;  // this lane's keys that the row does not attend
@@ -576,6 +585,7 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
         // the next tile's product beside this tile's weights (ahead of the other block's wave: 466 -> 456 us where the
         // matrix unit is the bound)
         __builtin_amdgcn_s_setprio(1);
+        locate(tile + 3);
         next = product(tile + 1);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -645,16 +655,17 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
 
     l += butterfly_partner<32>(l, lane);
     if (!live) return;
-    bool finish = !a.rec_o;
+    const auto &z = late<A>(a);  // arguments that the loop has no registers for
+    bool finish = !z.rec_o;
     if constexpr (PAGED) {
         finish = pieces <= 1;
-        if (!finish && piece == 0 && half == 0) a.records[orow] = pieces;
+        if (!finish && piece == 0 && half == 0) z.records[orow] = pieces;
     }
-    const size_t rec = orow * a.splits_total + a.split0 + piece;
-    float *to = finish ? a.out + orow * HD : a.rec_o + rec * HD;
+    const size_t rec = orow * z.splits_total + z.split0 + piece;
+    float *to = finish ? z.out + orow * HD : z.rec_o + rec * HD;
     const float inv = !finish ? 1.0f : l > 0 ? 1.0f / l : 0.0f;
     const bool none = finish && !(l > 0);  // nothing attended, or no softmax
-    if (!finish && half == 0) a.rec_ml[rec] = make_float2(M - kLift, l);
+    if (!finish && half == 0) z.rec_ml[rec] = make_float2(M - kLift, l);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
         const int d = DT * (8 * (j / 4) + 4 * half + j % 4);

@@ -6,7 +6,11 @@
 
 namespace nd {
 
-constexpr int kPagedSmall = 64;
+// Of how many rows blocks of 16 turn a request's keys over faster than blocks of 128 with few rows in them, for rows of 128,
+// 64 and 32 values: 64 requests of 2000 positions and 16, 32, 48 tokens of 4 rows each 188 against 205, 193 against 201, 191
+// against 179 us; 24, 48, 64 tokens 273 against 233, 281 against 207, 255 against 248. (With fewer blocks than compute units
+// up to twice as many rows.)
+inline int paged_small(int head_dim) { return head_dim == 32 ? 192 : head_dim == 64 ? 128 : 64; }
 
 // Requests of at most `small` rows (tokens times query heads per kv head) are in `row_tiles` blocks of 16 rows each, others
 // in blocks of 128 (`wide_blocks` of them at most).
@@ -20,15 +24,14 @@ inline PagedCut cut_paged(int cus, int head_dim, int requests, int tokens, int c
     PagedCut c;
     const int64_t rows = int64_t(count) * group;
     const int keys = window > 0 ? static_cast<int>(std::min<int64_t>(length, int64_t(window) + count - 1)) : length;
-    // Up to 64 rows, blocks of 16 turn a request's keys over faster than one block of 128 with few rows in it.
-    c.small = kPagedSmall;
+    c.small = paged_small(head_dim);
     if (rows <= c.small) {
         c.row_tiles = static_cast<int>((rows + kSpanRows - 1) / kSpanRows);
         c.rows = cut_span(cus, head_dim, rows, int64_t(requests) * kvheads, keys, keys, 2, false, false);
         return c;
     }
     static const SpanRate kFour[3] = {{4, 4, 5, 1.2, 1.6}, {4, 4, 5, 1.25, 2.4}, {4, 4, 5, 1.85, 4.1}};
-    static const SpanRate kWide[3] = {{4, 1, 6, 1.15, 1.5}, {4, 1, 6, 1.15, 1.7}, {4, 1, 6, 1.2, 2.3}};
+    static const SpanRate kWide[3] = {{4, 1, 6, 1.1, 1.27}, {4, 1, 6, 1.25, 1.45}, {4, 1, 6, 1.57, 2.2}};
     const int h = head_dim == 32 ? 0 : head_dim == 64 ? 1 : 2;
     const double row = 2.0 * (head_dim + 4);
     // every request has one, but only those with tokens and room for more of them have more

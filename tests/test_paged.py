@@ -97,11 +97,24 @@ def test_the_cut_holds_every_row(host, hd):
                     assert wide_blocks * wide_splits * kvheads < 1 << 23
 
 
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_the_tests_of_many_rows_reach_their_kernel(host, hd):
+    from tests.test_paged_wide_gpu import SHAPES, grown
+    for kvheads, group, counts, past in [*SHAPES, (1, 2, [90, 1, 130], [0]), (1, 2, [70, 1, 2, 40], [6000]), (1, 2, [80, 70, 66], [200]),
+                                         (1, 2, [70, 1], [150])]:
+        counts = grown(hd, group, counts)
+        v = (ct.c_int * 8)()
+        host.cut(hd, len(counts), sum(counts), max(counts), kvheads, group, max(past) + max(counts), 0, v)
+        small, row_tiles, _, _, _, wide_blocks, _, _ = v
+        assert wide_blocks and max(counts) * group > small, (kvheads, group, counts)
+        assert len(counts) == 1 or row_tiles * 16 >= small
+
+
 def test_argument_rules(host):
     assert host.pages_rule(1, 10, 16, 2, 64) is None and host.pages_rule(1, 2 ** 27 - 1, 16, 1, 32) is None
     for args, word in [((0, 10, 16, 2, 64), b"positive"), ((1, 0, 16, 2, 64), b"positive"), ((1, 10, 16, 0, 64), b"positive"),
                        ((1, 10, 8, 2, 64), b"page_size"), ((1, 10, 24, 2, 64), b"page_size"), ((1, 10, 512, 2, 64), b"page_size"),
-                       ((1, 10, 16, 2, 96), b"head_dim"), ((1, 10, 16, 70000, 64), b"65535"), ((1, 2 ** 27, 16, 2, 64), b"2^31")]:
+                       ((1, 10, 16, 2, 96), b"head_dim"), ((1, 10, 16, 70000, 64), b"65535"), ((1, 10, 256, 40000, 128), b"2^31 bytes"), ((1, 2 ** 27, 16, 2, 64), b"2^31")]:
         assert word in host.pages_rule(*args), args
     assert host.requests_rule(0, 1, 16) is None and host.requests_rule(8192, 2 ** 26, 16) is None
     for args, word in [((-1, 1, 16), b"8192"), ((8193, 1, 16), b"8192"), ((1, 0, 16), b"width"), ((1, 2 ** 26 + 1, 16), b"2^30")]:

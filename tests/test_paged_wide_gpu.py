@@ -10,6 +10,18 @@ from tests.test_paged_gpu import Batch, ints, upload
 pytestmark = pytest.mark.gpu
 
 
+# (kv heads, heads of each, new tokens, positions before them): grown(...) of them are in blocks of 128 rows
+SHAPES = [
+    (1, 1, [65], [0]), (1, 1, [129], [31]), (2, 2, [64, 100], [0, 500]), (1, 4, [32, 33, 1, 17, 16], [7, 0, 300, 64, 31]),
+    (2, 3, [43, 0, 86, 22], [1, 5, 33, 0]), (1, 8, [16, 9, 17, 8], [1000, 0, 3, 12]), (1, 16, [8, 9, 5, 4], [95, 96, 97, 0]),
+    (1, 5, [1, 26, 200, 1, 13, 14], [600, 0, 32, 0, 40, 41])]
+
+
+def grown(hd, group, counts):
+    """More tokens for narrower rows, of which more are in blocks of 16 rows."""
+    return [c * 128 // hd if c * group > 64 else c for c in counts]
+
+
 def some(rng, counts, n):
     """(request, token)s: the first and last of every request, those around blocks of 128 rows, and others."""
     rows = set()
@@ -20,13 +32,11 @@ def some(rng, counts, n):
 
 
 @pytest.mark.parametrize("hd", [32, 64, 128])
-@pytest.mark.parametrize("kvheads,group,counts,past", [
-    (1, 1, [65], [0]), (1, 1, [129], [31]), (2, 2, [64, 100], [0, 500]), (1, 4, [32, 33, 1, 17, 16], [7, 0, 300, 64, 31]),
-    (2, 3, [43, 0, 86, 22], [1, 5, 33, 0]), (1, 8, [16, 9, 17, 8], [1000, 0, 3, 12]), (1, 16, [8, 9, 5, 4], [95, 96, 97, 0]),
-    (1, 5, [1, 26, 200, 1, 13, 14], [600, 0, 32, 0, 40, 41])])
+@pytest.mark.parametrize("kvheads,group,counts,past", SHAPES)
 def test_pieces_and_decoding_requests(hd, kvheads, group, counts, past):
-    """Requests of 64 rows and fewer beside longer ones; blocks of one row and of all; fresh prompts and later pieces."""
+    """Requests of few rows beside longer ones; blocks of one row and of all; fresh prompts and later pieces."""
     rng = np.random.default_rng(hd + group + sum(counts))
+    counts = grown(hd, group, counts)
     b = Batch(rng, kvheads, group, hd, counts, past)
     got = b.run(tail=2)
     b.check(got[:-2], rows=some(rng, counts, 12), many=True)
@@ -45,7 +55,7 @@ def test_every_row_of_a_piece(hd, page):
 @pytest.mark.parametrize("window", [1, 16, 31, 32, 33, 100, 1000])
 def test_window(hd, window):
     rng = np.random.default_rng(hd + window)
-    counts = [90, 1, 130]
+    counts = grown(hd, 2, [90, 1, 130])
     b = Batch(rng, 1, 2, hd, counts, [0, 700, 333], page=32)
     b.check(b.run(window), window, rows=some(rng, counts, 30), many=True)
 
@@ -54,7 +64,7 @@ def test_window(hd, window):
 def test_pieces_of_long_contexts(hd):
     """Keys cut into pieces that are joined; row tiles with fewer pieces, requests with one, one that attends nothing."""
     rng = np.random.default_rng(hd)
-    counts = [70, 1, 2, 40]
+    counts = grown(hd, 2, [70, 1, 2, 40])
     b = Batch(rng, 1, 2, hd, counts, [6000, 3000, -1, 20], page=64)
     for length in (0, 100, 6070, 50000):
         got = b.run(length=length)
@@ -84,8 +94,8 @@ def test_many_requests(requests):
     rng = np.random.default_rng(requests)
     counts = [int(c) for c in rng.choice([0, 1, 2, 3], requests)]
     for r in rng.choice(requests, 5, replace=False):
-        counts[r] = int(rng.integers(65, 200))
-    counts[0], counts[-1] = 70, 99
+        counts[r] = int(rng.integers(193, 400))
+    counts[0], counts[-1] = 210, 299
     past = [int(p) for p in rng.integers(0, 40, requests)]
     b = Batch(rng, 1, 1, 32, counts, past)
     big = {(r, i) for r, c in enumerate(counts) if c > 60 for i in (0, 31, 64, c - 1)}
@@ -96,8 +106,9 @@ def test_many_requests(requests):
 @pytest.mark.parametrize("hd", [32, 64, 128])
 def test_pages_that_are_none(hd):
     rng = np.random.default_rng(hd)
-    counts = [80, 70, 66]
+    counts = grown(hd, 2, [80, 70, 66])
     b = Batch(rng, 1, 2, hd, counts, [200, 0, 40])
+    assert b.tables.shape[1] > 12
     whole = b.tables.copy()
     holes = [(0, 3), (0, 4), (0, 12), (1, 0), (1, 4)]
     for i, at in enumerate(holes):
@@ -115,7 +126,7 @@ def test_zero_rows_and_uneven_values(hd):
     """V rows of zeros, whose scale is 1, far above the others'; V scales that differ by powers of two; scores far apart;
     entries of q far above the rest over zero K codes."""
     rng = np.random.default_rng(hd)
-    b = Batch(rng, 1, 2, hd, [70, 1], [150, 90])
+    b = Batch(rng, 1, 2, hd, grown(hd, 2, [70, 1]), [150, 90])
     zero = rng.random(b.rows.vs.shape) < 0.1
     b.rows.v[zero], b.rows.vs[zero] = 0, 1.0
     b.rows.vs[~zero] *= 2.0 ** -rng.integers(0, 20, (~zero).sum())

@@ -395,13 +395,13 @@ int needle2_gpu_pages_reset(void *cache, void *stream);
  * pass its table or the batch, or that comes where the free pages no longer
  * suffice, gets none: its length stays, its first position is -1, and so are its
  * tokens' positions and slots, as are those behind the last request's. (One that
- * needs no new page is served all the same.) */
+ * needs no new page is served all the same.) No two of the arrays overlap. */
 int needle2_gpu_pages_extend(void *cache, int requests, const int *d_counts, int tokens, int *d_lengths, int *d_tables,
                              int width, int *d_starts, int *d_firsts, int *d_slots, int *d_positions, void *stream);
-/* Cuts request r to its first keep[r] positions (negative: 0; not longer than it
- * is): d_lengths is lowered, and the pages that hold none of them are free again
- * and -1 in d_tables. Right after an extension, a trim to the lengths before it
- * undoes it. Tables that hold pages which another request's table has too, or
+/* Cuts request r to its first keep[r] positions (negative: it stays as it is, and
+ * so does one that is not longer; 0: it ends): d_lengths is lowered, and the pages
+ * that hold none of them are free again and -1 in d_tables. Right after an
+ * extension, a trim to its d_firsts undoes it. Tables that hold pages which another request's table has too, or
  * that no extension dealt, are not for this call. */
 int needle2_gpu_pages_trim(void *cache, int requests, const int *d_keep, int *d_lengths, int *d_tables, int width,
                            void *stream);
@@ -417,7 +417,8 @@ int needle2_gpu_pages_store(void *cache, int layer, const float *d_k, int k_stri
  * x / sqrt(mean(x^2) + eps) * (1 + gain); then dimensions j and j + rotary / 2 are
  * turned by d_positions[token] * d_freq[j] (device fp64 [rotary / 2]; rotary 0:
  * not at all). head_dim 32, 64 or 128. Rows as in pages_store, of heads * head_dim
- * and kvheads * head_dim (0: none); outputs in place (the same stride) or apart.
+ * and kvheads * head_dim (0: none); outputs in place (with the same stride) or in
+ * memory of their own.
  * A token at a negative position (d_positions nullable without a rotation) is left
  * out, its outputs as they were. */
 int needle2_gpu_heads(const float *d_q, int q_stride, float *d_q_out, int q_out_stride, int heads, const float *d_k,

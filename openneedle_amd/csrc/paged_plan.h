@@ -24,7 +24,9 @@ inline PagedCut cut_paged(int cus, int head_dim, int requests, int tokens, int c
     PagedCut c;
     const int64_t rows = int64_t(count) * group;
     const int keys = window > 0 ? static_cast<int>(std::min<int64_t>(length, int64_t(window) + count - 1)) : length;
-    c.small = paged_small(head_dim);
+    // (a grid holds 2^24 blocks of 256 threads)
+    const int64_t most = std::max<int64_t>(1, (int64_t(1) << 22) / (int64_t(requests) * kvheads));
+    c.small = static_cast<int>(std::min<int64_t>(paged_small(head_dim), most * kSpanRows));
     if (rows <= c.small) {
         c.row_tiles = static_cast<int>((rows + kSpanRows - 1) / kSpanRows);
         c.rows = cut_span(cus, head_dim, rows, int64_t(requests) * kvheads, keys, keys, 2, false, false);
@@ -43,7 +45,7 @@ inline PagedCut cut_paged(int cus, int head_dim, int requests, int tokens, int c
         c.small = 0;
         return c;
     }
-    c.row_tiles = (c.small + kSpanRows - 1) / kSpanRows;
+    c.row_tiles = c.small / kSpanRows;
     best_cut(c.rows, cus, int64_t(requests) * kvheads, std::max(1, span_tiles(keys)), keys * row, kFour[h], 0.5, 3.5);
     return c;
 }

@@ -170,8 +170,8 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(ExtendArgs a) {
     if (t == 0) *a.free.top = top - taken;
 }
 
-// The pages of the positions from keep[r] on go back, the last one first, so that what an extension took lies in the stack
-// as before it.
+// The pages of the positions from keep[r] on go back (negative: none does), the last one first, so that what an extension
+// took lies in the stack as before it.
 __global__ __launch_bounds__(kThreads) void trim_kernel(TrimArgs a) {
     extern __shared__ int lds[];
     int *begin = lds, *left = lds + a.requests;  // pages that go back before r's; pages that r keeps
@@ -180,21 +180,24 @@ __global__ __launch_bounds__(kThreads) void trim_kernel(TrimArgs a) {
     const int top = *a.free.top;
     const int each = (a.requests + kThreads - 1) / kThreads;
     const int r0 = min(t * each, a.requests), r1 = min(r0 + each, a.requests);
-    auto kept = [&](int r, int &n) {
-        n = min(max(a.lengths[r], 0), most);
-        return min(max(a.keep[r], 0), n);
+    // n and what is kept of it, both within the table; true where the length is lowered
+    auto kept = [&](int r, int &n, int &k) {
+        const int length = a.lengths[r], keep = a.keep[r];
+        n = min(max(length, 0), most);
+        k = keep < 0 ? n : min(keep, n);
+        return keep >= 0 && length > keep;
     };
     Sums mine = {0, 0};
     for (int r = r0; r < r1; ++r) {
-        int n;
-        const int k = kept(r, n);
+        int n, k;
+        kept(r, n, k);
         mine.pages = capped(mine.pages, min(((n + page - 1) >> a.shift) - ((k + page - 1) >> a.shift), page_cap), page_cap);
     }
     Sums all;
     Sums at = scan(mine, 0, page_cap, all);
     for (int r = r0; r < r1; ++r) {
-        int n;
-        const int k = kept(r, n);
+        int n, k;
+        kept(r, n, k);
         begin[r] = at.pages;
         left[r] = (k + page - 1) >> a.shift;
         at.pages = capped(at.pages, min(((n + page - 1) >> a.shift) - left[r], page_cap), page_cap);
@@ -209,8 +212,8 @@ __global__ __launch_bounds__(kThreads) void trim_kernel(TrimArgs a) {
     }
     if (!ends_last(a.free.done)) return;
     for (int r = t; r < a.requests; r += kThreads) {
-        int n;
-        a.lengths[r] = kept(r, n);
+        int n, k;
+        if (kept(r, n, k)) a.lengths[r] = a.keep[r];
     }
     if (t == 0) *a.free.top = top + total;
 }

@@ -51,8 +51,9 @@ class PagedCache:
                                                  addr(d_slots), addr(d_positions), stream_ptr(stream)), "page extension")
 
     def trim(self, requests: int, d_keep, d_lengths, d_tables, width: int, stream=None) -> None:
-        """Cut every request to its first ``d_keep[r]`` positions (0: the request ends): pages that hold none of them are
-        free again and -1 in ``d_tables``. Only for tables whose pages :meth:`extend` dealt, each to one request."""
+        """Cut every request to its first ``d_keep[r]`` positions (0: the request ends; negative: it stays as it is): pages
+        that hold none of them are free again and -1 in ``d_tables``. With the ``d_firsts`` of an extension right before
+        it, it undoes that. Only for tables whose pages :meth:`extend` dealt, each to one request."""
         check(self._lib.needle2_gpu_pages_trim(self.ptr, int(requests), addr(d_keep), addr(d_lengths), addr(d_tables),
                                                int(width), stream_ptr(stream)), "page trim")
 

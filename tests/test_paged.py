@@ -75,9 +75,9 @@ def test_runs_hold_every_attended_position(host, tile, window):
 @pytest.mark.parametrize("hd", [32, 64, 128])
 def test_the_cut_holds_every_row(host, hd):
     """Blocks for every row, no more pieces than the join takes, no more blocks than a grid."""
-    for requests, counts in [(1, [1]), (1, [2000]), (64, [1] * 64), (8192, [1] * 8192), (7, [5] * 7), (51, [1] * 48 + [700, 3, 999]),
+    for requests, counts in [(1, [1]), (1, [2000]), (64, [1] * 64), (8192, [1] * 8192), (8192, [90] + [1] * 8191), (8192, [300] + [1] * 8191), (7, [5] * 7), (51, [1] * 48 + [700, 3, 999]),
                              (3, [0, 40, 0]), (2, [1, 100000])]:
-        for kvheads, group in ((1, 1), (4, 2), (8, 4), (2, 16), (1, 13)):
+        for kvheads, group in ((1, 1), (4, 2), (8, 4), (2, 16), (1, 13), (512, 1)):
             tokens, most = sum(counts), max(counts)
             if tokens * kvheads * group > 1 << 25:
                 continue
@@ -87,14 +87,13 @@ def test_the_cut_holds_every_row(host, hd):
                 small, row_tiles, splits, per, waves, wide_blocks, wide_splits, wide_per = v
                 assert splits >= 1 and per >= 1 and waves in (4, 8) and splits <= 1024
                 assert min(most * group, small) <= row_tiles * 16
-                assert row_tiles * requests * kvheads * splits < 1 << 22
+                assert (row_tiles * requests * splits + wide_blocks * wide_splits) * kvheads < 1 << 24
                 if most * group > small:
                     need, start = 0, 0
                     for r, c in enumerate(counts):
                         need = max(need, start * group // 128 + r + -(-c * group // 128))
                         start += c
                     assert wide_blocks >= need and 1 <= wide_splits <= 1024 and wide_per >= 1 and waves == 4
-                    assert wide_blocks * wide_splits * kvheads < 1 << 23
 
 
 @pytest.mark.parametrize("hd", [32, 64, 128])
@@ -163,7 +162,8 @@ def test_heads_refuses_before_any_launch():
 
     for args, word in [(dict(q=None), "null q"), (dict(qo=None), "null q"), (dict(k=None), "null k"), (dict(ko=None), "output of k"),
                        (dict(pos=None), "positions"), (dict(freq=None), "positions"), (dict(qs=252), "stride"), (dict(kos=130), "16 bytes"),
-                       (dict(k=at + 4), "16 bytes"), (dict(qg=at + 8), "gains"), (dict(rotary=65), "rotary"), (dict(hd=80), "head_dim")]:
+                       (dict(k=at + 4), "16 bytes"), (dict(qg=at + 8), "gains"), (dict(rotary=65), "rotary"), (dict(hd=80), "head_dim"),
+                       (dict(qo=at, qos=260), "one stride"), (dict(ko=at, kos=132), "one stride")]:
         assert heads(**args) == -1 and word in _ffi.last_error(), args
     assert heads(n=0, q=None, k=None, pos=None, freq=None) == 0
     assert heads(h=0, kvh=0, q=None, qo=None, k=None) == 0
@@ -206,7 +206,7 @@ class Pool:
     def trim(self, keep):
         gone = []
         for r, k in enumerate(keep):
-            k = min(max(k, 0), self.lengths[r])
+            k = self.lengths[r] if k < 0 else min(k, self.lengths[r])
             for i in range(-(-k // self.page), -(-self.lengths[r] // self.page)):
                 gone.append(self.tables[r][i])
                 self.tables[r][i] = -1
@@ -220,11 +220,15 @@ def test_the_model_of_the_tables():
     assert p.tables == [[0, 1, -1], [-1] * 3, [2, -1, -1]] and p.stack == [4, 3]
     before = [list(t) for t in p.tables], list(p.stack)
     p.extend([3, 4, -2], 8)
-    p.trim([5, 0, 1])
+    p.trim([5, -1, 1])
+    assert p.lengths == [5, 4, 1]
+    p.trim([9, 0, 2])
     assert ([list(t) for t in p.tables], p.stack) == before
     # the second gets none of two pages wanted where one is left, the third needs none
     p.extend([4, 0, 0], 8)
     assert p.extend([0, 5, 3], 8)[1] == [9, -1, 1] and p.lengths == [9, 0, 4] and len(p.stack) == 1
     assert p.extend([4, 0, 0], 8)[1] == [-1, 0, 4]  # past its table
     p.trim([0, 9, -1])
+    assert p.lengths == [0, 0, 4]
+    p.trim([0, 0, 0])
     assert p.lengths == [0, 0, 0] and sorted(p.stack) == [0, 1, 2, 3, 4]

@@ -79,12 +79,13 @@ def test_tables_of_many_requests(requests, most):
 
 def test_extension_undone_by_trim():
     """A trim to the lengths before it leaves the stack of free pages as it was: the next extension deals the same."""
-    t = Tables(200, 16, 40, 12)
+    t = Tables(150, 16, 40, 12)
     t.extend(np.arange(40) % 50, 2000)
     t.trim(np.arange(40) // 2)
     before, stack = list(t.model.lengths), list(t.model.stack)
     a = t.extend(np.full(40, 21), 840)
-    t.trim(before)
+    t.trim(a[1])  # the first positions: -1 where a request got nothing
+    assert t.model.lengths == before
     assert t.model.stack == stack
     for x, y in zip(a, t.extend(np.full(40, 21), 840)):
         np.testing.assert_array_equal(x, y)
@@ -118,6 +119,8 @@ def test_tables_that_were_not_dealt_are_safe():
     kv.extend(4, ints([0, 0, 0, 15]), 15, lengths, ints([[0, 1], [2, 3], [4, 5], [99, 600]]), 2, out[0], out[1],
               *(ints(np.zeros(15)) for _ in "sp"))
     synchronize()
+    kv.trim(4, ints([-1, -7, 2 ** 31 - 1, 20]), lengths, tables, 2)  # (the last one has 17 + 15)
+    np.testing.assert_array_equal(lengths.to_host(np.int32, 4), [-5, 33, 2 ** 31 - 1, 20])
     many = ints([[9, 9, 9]] * 9)
     kv.trim(9, ints([0] * 9), ints([48] * 9), many, 3)
     assert kv.free_pages() == 6

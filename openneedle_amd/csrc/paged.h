@@ -66,6 +66,10 @@ struct PagedSpanArgs : SpanArgs {
     const int *starts, *tables;
     int tokens, width;
     int small, row_tiles;
+    // Not 0: the requests in blocks of 16 rows are taken by their lengths, the longest first, in rounds of so many of which
+    // every other goes from the shortest up: blocks that share a compute unit, a round's and the next one's, then have
+    // about as much to do as other pairs.
+    int round;
     int wide_splits, wide_per;
     int wide_blocks;       // of 128 rows, an upper bound
     int *records;          // [rows]: a row's records where it has several (0 before the call, and after the join)

@@ -261,6 +261,7 @@ int needle2_gpu_pages_attention(void *h, int layer, const float *d_q, float *d_o
         const PagedCut cut = cut_paged(device_cus(), p.head_dim, requests, tokens, count, p.kvheads, a.group, most, window);
         a.small = cut.small;
         a.row_tiles = cut.row_tiles;
+        a.round = cut.round;
         a.splits = cut.rows.splits;
         a.per = cut.rows.per;
         a.waves = cut.rows.waves;

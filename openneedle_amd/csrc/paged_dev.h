@@ -50,6 +50,43 @@ __device__ __forceinline__ WideBlock wide_block(const PagedSpanArgs &a, int b, i
     return WideBlock{low, max(0, b - __builtin_amdgcn_readfirstlane(from(low))) * kWideRows};
 }
 
+// The request with the k-th most positions before its tokens (of equal ones in a fixed order), by one wave, of at most
+// kRanked requests: a search for that number of positions, bit by bit, by counting the requests that reach it.
+__device__ __forceinline__ int ranked_request(const PagedSpanArgs &a, int k, int lane) {
+    constexpr int kEach = kRanked / 64;
+    const ND_GLOBAL int *firsts = (const ND_GLOBAL int *)(a.positions);
+    const int most = a.width << a.pool.shift;
+    int past[kEach];  // one more than it has; -1: no request
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int r = i * 64 + lane;
+        past[i] = -1;
+        if (i * 64 < a.units) past[i] = r < a.units ? max(min(firsts[min(r, a.units - 1)], most), -1) + 1 : -1;
+    }
+    auto reach = [&](int limit) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (i * 64 < a.units) n += __popcll(__ballot(past[i] >= limit));
+        return n;
+    };
+    int value = 0;  // the largest that more than k of them reach
+    for (int bit = 31 - __builtin_clz(most + 1); bit >= 0; --bit)
+        if (reach(value + (1 << bit)) > k) value += 1 << bit;
+    k -= reach(value + 1);
+    int found = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const uint64_t equal = __ballot(past[i] == value);
+        const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(equal >> 32),
+                                                     __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(equal), 0));
+        const uint64_t it = __ballot(past[i] == value && before == k);
+        if (it) found = i * 64 + __builtin_ctzll(it);
+        k -= __popcll(equal);
+    }
+    return __builtin_amdgcn_readfirstlane(found);
+}
+
 // The pages of a request and kv head. A page outside the cache is none (-1): its rows read as zeros and are masked.
 template <int HD>
 struct PageReader {

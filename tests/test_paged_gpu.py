@@ -312,7 +312,10 @@ def test_several_pieces(hd, length):
     b.check(b.run(window=900, length=length), 900)
 
 
-@pytest.mark.parametrize("requests,kvheads", [(40, 8), (64, 5), (65, 4), (130, 3), (511, 1)])
+ORDERED = [(40, 8), (64, 5), (65, 4), (130, 3), (511, 1)]  # requests and kv heads
+
+
+@pytest.mark.parametrize("requests,kvheads", ORDERED)
 def test_requests_in_the_order_of_their_lengths(requests, kvheads):
     """More blocks than compute units: every request is taken once, whatever lengths they share, tokens or not, padded or
     past their tables."""
@@ -320,15 +323,16 @@ def test_requests_in_the_order_of_their_lengths(requests, kvheads):
     past = [int(x) for x in rng.choice([0, 1, 60, 61, 61, 61, 200, 300, 300, 1100, -1, -7], requests)]
     counts = [int(c) for c in rng.choice([1, 1, 1, 1, 2, 0], requests)]
     b = Batch(rng, kvheads, 2, 32, counts, past, page=32)
-    got = b.run(length=1200)
+    assert b.width * 32 >= 1152
+    got = b.run(length=1152)
     assert np.isfinite(got).all()
     b.check(got)
     firsts = list(past)
     firsts[3], firsts[-2] = 2 ** 31 - 1, 32 * b.width
     b.past = [p if f == p else -1 for p, f in zip(past, firsts)]
-    b.check(b.run(length=1200, firsts=firsts))
-    same = Batch(rng, kvheads, 2, 32, [1] * requests, [77] * requests, page=32)
-    same.check(same.run(length=1200))
+    b.check(b.run(length=1152, firsts=firsts))
+    same = Batch(rng, kvheads, 2, 32, [1] * requests, [77] * requests, page=32, extra_width=40)
+    same.check(same.run(length=1152))
 
 
 def test_the_same_numbers_again():

@@ -48,9 +48,11 @@ inline PagedCut cut_paged(int cus, int head_dim, int requests, int tokens, int c
     static const SpanRate kWide[3] = {{4, 1, 6, 1.1, 1.27}, {4, 1, 6, 1.25, 1.45}, {4, 1, 6, 1.57, 2.2}};
     const int h = head_dim == 32 ? 0 : head_dim == 64 ? 1 : 2;
     const double row = 2.0 * (head_dim + 4);
-    // every request has one, but only those with tokens and room for more of them have more
-    c.wide_blocks = static_cast<int>(int64_t(tokens) * group / kWideRows) + requests;
-    const int64_t filled = std::max<int64_t>(1, int64_t(tokens) * group / kWideRows);
+    // the tokens' whole blocks, and one that is not filled for every request that may have more than `small` rows (every
+    // one where they are found without their lengths)
+    const int64_t whole = int64_t(tokens) * group / kWideRows, filled = std::max<int64_t>(1, whole);
+    c.wide_blocks = static_cast<int>(whole + (requests > kRanked ? requests
+                                                                 : std::min<int64_t>(requests, int64_t(tokens) * group / (c.small + 1) + 1)));
     const double record = double(tokens) * group * kvheads * head_dim * 8 / 3e6;
     best_cut(c.wide, cus, filled * kvheads, std::max(1, wide_tiles(keys)), keys * row, kWide[h], record, 3.5);
     if (requests == 1) {  // (whatever its tokens turn out to be)

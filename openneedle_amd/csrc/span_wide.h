@@ -140,11 +140,12 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
     Request req;
     if constexpr (PAGED) {
         kh = bx % a.kvheads;
-        // the last row tiles, which attend the most, first
-        const WideBlock b = wide_block(a, a.wide_blocks - 1 - bx / a.kvheads % a.wide_blocks, lane);
+        const int at = bx / a.kvheads % a.wide_blocks;
+        const WideBlock b = a.units <= kRanked ? ranked_block(a, at, lane) : wide_block(a, a.wide_blocks - 1 - at, lane);
         piece = bx / a.kvheads / a.wide_blocks;
         unit = b.unit;
         tile_rows = b.row;
+        if (tile_rows < 0) return;
         req = request(a, unit);
         rows = req.count * a.group;
         if (rows <= a.small || tile_rows >= rows) return;

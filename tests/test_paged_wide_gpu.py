@@ -88,15 +88,18 @@ def test_one_request_of_fewer_tokens_than_announced():
     assert np.isnan(b.run(count=200, tail=200)).all()
 
 
-@pytest.mark.parametrize("requests", [63, 64, 65, 700])
+@pytest.mark.parametrize("requests", [63, 64, 65, 300, 512, 513, 700])
 def test_many_requests(requests):
-    """Blocks find their requests among more than a wave looks at at once; most of them have no tokens, or few."""
+    """Blocks find their requests among more than a wave looks at at once; most of them have no tokens, or few; some are of
+    the same length, one is padded."""
     rng = np.random.default_rng(requests)
     counts = [int(c) for c in rng.choice([0, 1, 2, 3], requests)]
     for r in rng.choice(requests, 5, replace=False):
         counts[r] = int(rng.integers(193, 400))
     counts[0], counts[-1] = 210, 299
     past = [int(p) for p in rng.integers(0, 40, requests)]
+    counts[20:23], past[20:23] = [257] * 3, [33] * 3
+    counts[40], past[40] = 250, -3
     b = Batch(rng, 1, 1, 32, counts, past)
     big = {(r, i) for r, c in enumerate(counts) if c > 60 for i in (0, 31, 64, c - 1)}
     small = {(r, i) for r, c in enumerate(counts[:60]) if c <= 60 for i in range(c)}

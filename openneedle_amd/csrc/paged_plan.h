@@ -44,6 +44,9 @@ inline PagedCut cut_paged(int cus, int head_dim, int requests, int tokens, int c
         if (by_length(cus, requests, blocks, keys)) c.round = std::max(1, cus / kvheads);
         return c;
     }
+    // Beside blocks of 128, at most four blocks of 16 a request, most of which have no rows (500 decoding requests and a
+    // prompt piece, rows of 64 values: eight 112 us, four 96, two 90).
+    c.small = std::min(c.small, 64);
     static const SpanRate kFour[3] = {{4, 4, 5, 1.2, 1.6}, {4, 4, 5, 1.25, 2.4}, {4, 4, 5, 1.85, 4.1}};
     static const SpanRate kWide[3] = {{4, 1, 6, 1.1, 1.27}, {4, 1, 6, 1.25, 1.45}, {4, 1, 6, 1.57, 2.2}};
     const int h = head_dim == 32 ? 0 : head_dim == 64 ? 1 : 2;

@@ -157,7 +157,7 @@ template <int HD, int ROWS, int ROT>
 void launch_rows(const HeadsArgs &a, int all, hipStream_t s) {
     const int parts = (all + ROWS - 1) / ROWS, per_block = 256 / (HD / 4);
     const int64_t items = static_cast<int64_t>(a.tokens) * parts;
-    ND_CHECK(items < (int64_t(1) << 31), "heads: more than 2^31 parts of rows");
+    ND_CHECK(items * (HD / 4) < (int64_t(1) << 32) - 256, "heads: more rows than a grid holds");
     hipLaunchKernelGGL((heads_kernel<HD, ROWS, ROT>), dim3(static_cast<unsigned>((items + per_block - 1) / per_block)),
                        dim3(256), 0, s, a, parts);
     ND_HIP(hipGetLastError());

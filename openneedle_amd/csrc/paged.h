@@ -34,7 +34,7 @@ struct TrimArgs {
     int *lengths, *tables;
     int requests, width, shift;
 };
-void launch_zero(int *at, size_t n, hipStream_t s);
+void launch_zero(int2 *at, size_t n, hipStream_t s);
 void launch_pages_reset(const PageStack &f, hipStream_t s);
 void launch_extend(const ExtendArgs &a, hipStream_t s);
 void launch_trim(const TrimArgs &a, hipStream_t s);
@@ -72,10 +72,16 @@ struct PagedSpanArgs : SpanArgs {
     int round;
     int wide_splits, wide_per;
     int wide_blocks;       // of 128 rows, an upper bound
-    int *records;          // [rows]: a row's records where it has several (0 before the call, and after the join)
+    // Where there may be several pieces: how many records a row has, and its row of out; 0 before the call, and after the
+    // join. Rows in blocks of 16, [units][kvheads][16 row_tiles], with rec_o, rec_ml and splits_total (= splits); those in
+    // blocks of 128 as in q, with records of their own, wide_splits a row.
+    int2 *some, *wide_some;
+    float *wide_o;
+    float2 *wide_ml;
 };
 // `waves` and the pieces by splits, per; wide: the blocks of 128 rows too
 void launch_paged(const PagedSpanArgs &a, int head_dim, hipStream_t s);
-void launch_paged_join(const PagedSpanArgs &a, int head_dim, hipStream_t s);
+// The records of `rows` rows: rec_o, rec_ml, splits_total and some of `a`.
+void launch_paged_join(const PagedSpanArgs &a, int64_t rows, int head_dim, hipStream_t s);
 
 }  // namespace nd

@@ -16,7 +16,7 @@ struct PagedHandle {
     DevBuf<uint8_t> rows;
     DevBuf<int> stack, state;  // state: free pages; blocks of a running launch that are done
     KeptBuf<float> records;    // of the attention (span.h)
-    KeptBuf<int> numbers;
+    KeptBuf<int2> some;
 
     size_t layer_bytes() const { return size_t(pages) * kvheads * page_block_bytes(shift, head_dim); }
     PageStack free() const { return PageStack{stack.p, state.p, state.p + 1, pages}; }
@@ -268,17 +268,29 @@ int needle2_gpu_pages_attention(void *h, int layer, const float *d_q, float *d_o
         a.wide_blocks = cut.wide_blocks;
         a.wide_splits = cut.wide.splits;
         a.wide_per = cut.wide.per;
-        a.splits_total = std::max(cut.row_tiles ? a.splits : 1, cut.wide_blocks ? a.wide_splits : 1);
-        if (a.splits_total > 1) {
-            const size_t rows = size_t(tokens) * heads, n = rows * a.splits_total;
-            a.rec_o = p.records.reserve(n * (p.head_dim + 2));
-            a.rec_ml = reinterpret_cast<float2 *>(a.rec_o + n * p.head_dim);
-            const int *before = p.numbers.bufs.empty() ? nullptr : p.numbers.bufs.back()->p;
-            a.records = p.numbers.reserve(rows);
-            if (a.records != before) launch_zero(a.records, p.numbers.bufs.back()->n, s);
+        a.splits_total = a.splits;
+        const size_t few = size_t(cut.few_records), many = size_t(cut.wide_records);
+        if (few + many) {
+            const size_t n = few * a.splits, m = many * a.wide_splits;
+            a.rec_o = p.records.reserve((n + m) * (p.head_dim + 2));
+            a.wide_o = a.rec_o + n * p.head_dim;
+            a.rec_ml = reinterpret_cast<float2 *>(a.wide_o + m * p.head_dim);
+            a.wide_ml = a.rec_ml + n;
+            const int2 *before = p.some.bufs.empty() ? nullptr : p.some.bufs.back()->p;
+            a.some = p.some.reserve(few + many);
+            a.wide_some = a.some + few;
+            if (a.some != before) launch_zero(a.some, p.some.bufs.back()->n, s);
         }
         launch_paged(a, p.head_dim, s);
-        if (a.splits_total > 1) launch_paged_join(a, p.head_dim, s);
+        if (few) launch_paged_join(a, int64_t(few), p.head_dim, s);
+        if (many) {
+            PagedSpanArgs w = a;
+            w.rec_o = a.wide_o;
+            w.rec_ml = a.wide_ml;
+            w.some = a.wide_some;
+            w.splits_total = a.wide_splits;
+            launch_paged_join(w, int64_t(many), p.head_dim, s);
+        }
     });
 }
 

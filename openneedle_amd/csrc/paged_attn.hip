@@ -39,7 +39,7 @@ template <int HD, int G>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedSpanArgs a, int64_t rows) {
     constexpr int kRows = 256 / (G * (HD / 4));
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
-    join_rows<HD, G, true>(a, row0, static_cast<int>(min(static_cast<int64_t>(kRows), rows - row0)), a.records);
+    join_rows<HD, G, true>(a, row0, static_cast<int>(min(static_cast<int64_t>(kRows), rows - row0)), a.some);
 }
 
 template <int HD>
@@ -66,9 +66,8 @@ void launch_paged(const PagedSpanArgs &a, int head_dim, hipStream_t s) {
     }
 }
 
-void launch_paged_join(const PagedSpanArgs &a, int head_dim, hipStream_t s) {
+void launch_paged_join(const PagedSpanArgs &a, int64_t rows, int head_dim, hipStream_t s) {
     ND_CHECK(a.splits_total <= kJoinMax, "attention: too many pieces");
-    const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
     with_join(head_dim, a.splits_total, [&](auto hd, auto groups) {
         constexpr int HD = decltype(hd)::value, G = decltype(groups)::value;
         constexpr int kRows = 256 / (G * (HD / 4));

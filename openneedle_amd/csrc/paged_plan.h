@@ -27,9 +27,11 @@ struct PagedCut {
     int small = 0, row_tiles = 0, wide_blocks = 0;
     int round = 0;  // blocks of 16 rows by length (paged.h: PagedSpanArgs)
     SpanCut rows, wide;
+    // rows that have rows.splits and wide.splits records each (0: one piece)
+    int64_t few_records = 0, wide_records = 0;
 };
 
-inline PagedCut cut_paged(int cus, int head_dim, int requests, int tokens, int count, int kvheads, int group, int length,
+inline PagedCut cut_paged_blocks(int cus, int head_dim, int requests, int tokens, int count, int kvheads, int group, int length,
                           int window) {
     PagedCut c;
     const int64_t rows = int64_t(count) * group;
@@ -64,6 +66,14 @@ inline PagedCut cut_paged(int cus, int head_dim, int requests, int tokens, int c
     }
     c.row_tiles = c.small / kSpanRows;
     best_cut(c.rows, cus, int64_t(requests) * kvheads, std::max(1, span_tiles(keys)), keys * row, kFour[h], 0.5, 3.5);
+    return c;
+}
+
+inline PagedCut cut_paged(int cus, int head_dim, int requests, int tokens, int count, int kvheads, int group, int length,
+                          int window) {
+    PagedCut c = cut_paged_blocks(cus, head_dim, requests, tokens, count, kvheads, group, length, window);
+    if (c.row_tiles && c.rows.splits > 1) c.few_records = int64_t(requests) * kvheads * c.row_tiles * kSpanRows;
+    if (c.wide_blocks && c.wide.splits > 1) c.wide_records = int64_t(tokens) * kvheads * group;
     return c;
 }
 

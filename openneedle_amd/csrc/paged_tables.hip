@@ -78,9 +78,9 @@ __device__ __forceinline__ bool ends_last(int *done) {
     return last;
 }
 
-__global__ __launch_bounds__(256) void zero_kernel(int *at, size_t n) {
+__global__ __launch_bounds__(256) void zero_kernel(int2 *at, size_t n) {
     const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (i < n) at[i] = 0;
+    if (i < n) at[i] = make_int2(0, 0);
 }
 
 __global__ __launch_bounds__(256) void pages_reset_kernel(PageStack f) {
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(kThreads) void trim_kernel(TrimArgs a) {
 
 }  // namespace
 
-void launch_zero(int *at, size_t n, hipStream_t s) {
+void launch_zero(int2 *at, size_t n, hipStream_t s) {
     hipLaunchKernelGGL(zero_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s, at, n);
     ND_HIP(hipGetLastError());
 }

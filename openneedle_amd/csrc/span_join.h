@@ -36,9 +36,10 @@ __device__ __forceinline__ float2 join_sums(const SpanArgs &a, size_t row, int n
 // (every G-th each), whose loads do not wait for each other; 256 / (G * HD / 4) rows at a time. The sums' order depends
 // on the number of records only. Latency bounds it: 64 x 32 rows of 128 values 5 us, a long prefix's many records 7.
 constexpr int kJoinMax = 1024;  // records of a row
-// SOME: rows have records[row] of them, from 2 on; 0: the row is left as it is. Read, they are 0 again for the next call.
+// SOME: row r has some[r].x of them, from 2 on, and is row some[r].y of the output; of 0 there is nothing to join. What is
+// read is 0 again for the next call.
 template <int HD, int G, bool SOME = false>
-__device__ __forceinline__ void join_rows(const SpanArgs &a, size_t row0, int count, int *records = nullptr) {
+__device__ __forceinline__ void join_rows(const SpanArgs &a, size_t row0, int count, int2 *some = nullptr) {
     constexpr int kLanes = HD / 4, kRows = 256 / (G * kLanes);
     constexpr int kFactors = kRows * (G == 8 ? kJoinMax : G);
     __shared__ float factor[kFactors];
@@ -46,16 +47,17 @@ __device__ __forceinline__ void join_rows(const SpanArgs &a, size_t row0, int co
     __shared__ __attribute__((aligned(16))) float part[G > 1 ? G : 1][kRows][HD];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int splits = a.splits_total;
-    __shared__ int number[SOME ? kRows : 1];
+    __shared__ int2 number[SOME ? kRows : 1];
     const int d = t % kLanes * 4, g = t / kLanes % G, r = t / (kLanes * G);
     for (int i0 = 0; i0 < count; i0 += kRows) {
         for (int i = wave; i < kRows && i0 + i < count; i += 4) {
             int n = splits;
             if constexpr (SOME) {
-                n = min(__builtin_amdgcn_readfirstlane(records[row0 + i0 + i]), splits);
-                if (lane == 0) number[i] = n;
+                const int2 its = some[row0 + i0 + i];
+                n = min(__builtin_amdgcn_readfirstlane(its.x), splits);
+                if (lane == 0) number[i] = make_int2(n, its.y);
                 if (n == 0) continue;
-                if (lane == 0) records[row0 + i0 + i] = 0;
+                if (lane == 0) some[row0 + i0 + i].x = 0;
             }
             const float2 all = join_sums(a, row0 + i0 + i, n, lane, factor + i * splits);
             if (lane == 0) total[i] = all.y;
@@ -63,9 +65,11 @@ __device__ __forceinline__ void join_rows(const SpanArgs &a, size_t row0, int co
         __syncthreads();
         bool live = i0 + r < count;
         int n = splits;
+        size_t to = row0 + i0 + r;
         if constexpr (SOME) {
-            n = live ? number[r] : 0;
+            n = live ? number[r].x : 0;
             live = n > 0;
+            if (live) to = number[r].y;
         }
         float4 o = make_float4(0, 0, 0, 0);
         if (live) {
@@ -97,7 +101,7 @@ __device__ __forceinline__ void join_rows(const SpanArgs &a, size_t row0, int co
         }
         if (live && g == 0) {
             const float L = total[r], inv = 1.0f / L;
-            *reinterpret_cast<float4 *>(a.out + (row0 + i0 + r) * HD + d) =
+            *reinterpret_cast<float4 *>(a.out + to * HD + d) =
                 L > 0 ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0, 0, 0, 0);
         }
         __syncthreads();

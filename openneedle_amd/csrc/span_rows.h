@@ -387,7 +387,9 @@ __device__ __forceinline__ void span_rows(const A &a, int bx, int kh, int unit) 
     bool finish = !a.rec_o;
     if constexpr (PAGED) {
         finish = pieces <= 1;
-        if (!finish && piece == 0 && wave == 0 && quad == 0 && live) a.records[orow] = pieces;
+        if (!finish && piece == 0 && wave == 0 && quad == 0 && live)
+            a.some[(static_cast<size_t>(unit) * a.kvheads + kh) * (a.row_tiles * kSpanRows) + row] =
+                make_int2(pieces, static_cast<int>(orow));
     }
     if (quad == 0) {
         sm[wave][col] = m;
@@ -426,7 +428,9 @@ __device__ __forceinline__ void span_rows(const A &a, int bx, int kh, int unit) 
             *reinterpret_cast<float4 *>(a.out + at * HD + d) =
                 L > 0 ? make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv) : make_float4(0, 0, 0, 0);
         } else {
-            const size_t rec = at * a.splits_total + a.split0 + piece;
+            size_t rec = at * a.splits_total + a.split0 + piece;
+            if constexpr (PAGED)
+                rec = ((static_cast<size_t>(unit) * a.kvheads + kh) * (a.row_tiles * kSpanRows) + grow) * a.splits_total + piece;
             *reinterpret_cast<float4 *>(a.rec_o + rec * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
             if (d == 0) a.rec_ml[rec] = make_float2(M, L);
         }

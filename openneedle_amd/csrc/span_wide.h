@@ -660,13 +660,24 @@ __device__ __forceinline__ void span_wide(const A &a, int bx) {
     bool finish = !z.rec_o;
     if constexpr (PAGED) {
         finish = pieces <= 1;
-        if (!finish && piece == 0 && half == 0) z.records[orow] = pieces;
+        if (!finish && piece == 0 && half == 0) z.wide_some[orow] = make_int2(pieces, static_cast<int>(orow));
     }
-    const size_t rec = orow * z.splits_total + z.split0 + piece;
-    float *to = finish ? z.out + orow * HD : z.rec_o + rec * HD;
+    size_t rec;
+    float *rec_o;
+    float2 *rec_ml;
+    if constexpr (PAGED) {
+        rec = orow * z.wide_splits + piece;
+        rec_o = z.wide_o;
+        rec_ml = z.wide_ml;
+    } else {
+        rec = orow * z.splits_total + z.split0 + piece;
+        rec_o = z.rec_o;
+        rec_ml = z.rec_ml;
+    }
+    float *to = finish ? z.out + orow * HD : rec_o + rec * HD;
     const float inv = !finish ? 1.0f : l > 0 ? 1.0f / l : 0.0f;
     const bool none = finish && !(l > 0);  // nothing attended, or no softmax
-    if (!finish && half == 0) z.rec_ml[rec] = make_float2(M - kLift, l);
+    if (!finish && half == 0) rec_ml[rec] = make_float2(M - kLift, l);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
         const int d = DT * (8 * (j / 4) + 4 * half + j % 4);

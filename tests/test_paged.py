@@ -26,8 +26,9 @@ void runs(int first, int last, int window, int tile, int *out) {
 }
 void cut(int hd, int requests, int tokens, int count, int kvheads, int group, int length, int window, int *out) {
     nd::PagedCut c = nd::cut_paged(256, hd, requests, tokens, count, kvheads, group, length, window);
-    int v[9] = {c.small, c.row_tiles, c.rows.splits, c.rows.per, c.rows.waves, c.wide_blocks, c.wide.splits, c.wide.per, c.round};
-    for (int i = 0; i < 9; ++i) out[i] = v[i];
+    int v[10] = {c.small, c.row_tiles, c.rows.splits, c.rows.per, c.rows.waves, c.wide_blocks, c.wide.splits, c.wide.per, c.round,
+                 int(c.few_records * c.rows.splits + c.wide_records * c.wide.splits)};
+    for (int i = 0; i < 10; ++i) out[i] = v[i];
 }
 const char *pages_rule(int l, int n, int p, int k, int d) { return nd::check_pages(l, n, p, k, d); }
 const char *requests_rule(int r, int w, int p) { return nd::check_requests(r, w, p); }
@@ -76,18 +77,19 @@ def test_runs_hold_every_attended_position(host, tile, window):
 def test_the_cut_holds_every_row(host, hd):
     """Blocks for every row, no more pieces than the join takes, no more blocks than a grid."""
     for requests, counts in [(1, [1]), (1, [2000]), (64, [1] * 64), (8192, [1] * 8192), (8192, [90] + [1] * 8191), (8192, [300] + [1] * 8191), (7, [5] * 7), (51, [1] * 48 + [700, 3, 999]),
-                             (3, [0, 40, 0]), (2, [1, 100000])]:
+                             (3, [0, 40, 0]), (2, [1, 100000]), (2, [1, 8000]), (3, [1, 60, 3000])]:
         for kvheads, group in ((1, 1), (4, 2), (8, 4), (2, 16), (1, 13), (512, 1)):
             tokens, most = sum(counts), max(counts)
             if tokens * kvheads * group > 1 << 25:
                 continue
             for length, window in ((max(1, most), 0), (8192 + most, 0), (1 << 20, 0), (1 << 20, 500)):
-                v = (ct.c_int * 9)()
+                v = (ct.c_int * 10)()
                 host.cut(hd, requests, tokens, most, kvheads, group, length, window, v)
-                small, row_tiles, splits, per, waves, wide_blocks, wide_splits, wide_per, round = v
+                small, row_tiles, splits, per, waves, wide_blocks, wide_splits, wide_per, round, records = v
                 assert splits >= 1 and per >= 1 and waves in (4, 8) and splits <= 1024
                 assert min(most * group, small) <= row_tiles * 16
                 assert round == 0 or requests <= 512
+                assert 0 <= records <= 1 << 18  # of the scratch: 140 MB at most
                 assert (row_tiles * requests * splits + wide_blocks * wide_splits) * kvheads < 1 << 24
                 if most * group > small:
                     need, start = 0, 0
@@ -106,9 +108,9 @@ def test_the_tests_of_many_rows_reach_their_kernel(host, hd):
     for kvheads, group, counts, past in [*SHAPES, (1, 2, [90, 1, 130], [0]), (1, 2, [70, 1, 2, 40], [6000]), (1, 2, [80, 70, 66], [200]),
                                          (1, 2, [70, 1], [150])]:
         counts = grown(hd, group, counts)
-        v = (ct.c_int * 9)()
+        v = (ct.c_int * 10)()
         host.cut(hd, len(counts), sum(counts), max(counts), kvheads, group, max(past) + max(counts), 0, v)
-        small, row_tiles, _, _, _, wide_blocks, _, _, _ = v
+        small, row_tiles, _, _, _, wide_blocks, *_ = v
         assert wide_blocks and max(counts) * group > small, (kvheads, group, counts)
         assert len(counts) == 1 or row_tiles * 16 >= small
 
@@ -117,7 +119,7 @@ def test_the_tests_of_ordered_requests_reach_the_order(host):
     from tests.test_paged_gpu import ORDERED
     for requests, kvheads in ORDERED:
         for count in (1, 2):
-            v = (ct.c_int * 9)()
+            v = (ct.c_int * 10)()
             host.cut(32, requests, requests * count, count, kvheads, 2, 1152, 0, v)
             assert v[8] > 0, (requests, kvheads)
     host.cut(64, 1, 1, 1, 1, 2, 1 << 20, 0, v)

@@ -395,7 +395,8 @@ int needle2_gpu_pages_reset(void *cache, void *stream);
  * pass its table or the batch, or that comes where the free pages no longer
  * suffice, gets none: its length stays, its first position is -1, and so are its
  * tokens' positions and slots, as are those behind the last request's. (One that
- * needs no new page is served all the same.) No two of the arrays overlap. */
+ * needs no new page is served all the same, but none behind one that passes the
+ * batch.) No two of the arrays overlap. */
 int needle2_gpu_pages_extend(void *cache, int requests, const int *d_counts, int tokens, int *d_lengths, int *d_tables,
                              int width, int *d_starts, int *d_firsts, int *d_slots, int *d_positions, void *stream);
 /* Cuts request r to its first keep[r] positions (negative: it stays as it is, and

@@ -269,6 +269,10 @@ int needle2_gpu_pages_attention(void *h, int layer, const float *d_q, float *d_o
         a.wide_splits = cut.wide.splits;
         a.wide_per = cut.wide.per;
         a.splits_total = a.splits;
+        if (length == 0) {  // cut for the tables' width: requests that are far shorter have pieces of their own size
+            a.per = std::min(a.per, 2 * a.waves);
+            a.wide_per = std::min(a.wide_per, 16);
+        }
         const size_t few = size_t(cut.few_records), many = size_t(cut.wide_records);
         if (few + many) {
             const size_t n = few * a.splits, m = many * a.wide_splits;

@@ -1,5 +1,5 @@
-// How the paged attention's launch is cut, as arithmetic on plain integers (no HIP types: tested on any host), by the
-// estimates of span_plan.h.
+// How the paged attention's launch is cut, as arithmetic on plain integers (no HIP types: tested on any host), by
+// estimates as span_plan.h's.
 #pragma once
 
 #include "span_plan.h"
@@ -31,17 +31,31 @@ struct PagedCut {
     int64_t few_records = 0, wide_records = 0;
 };
 
+// us that one piece more costs blocks of 16 rows (one request of 60000 positions, rows of 32 values: 32, 64 and 118 pieces
+// 20.2, 17.7 and 17.0 us). At span_plan.h's 0.5 requests were cut too coarsely: one of 1500, 8000 and 30000 positions, rows
+// of 64, took 13.1, 14.6 and 20.9 us and takes 10.5, 11.6 and 17.4; one of 4000, rows of 128, 16.4 and 13.3; but twelve of
+// 600 there 14.1 and 15.3.
+constexpr double kPiece = 0.03;
+
 inline PagedCut cut_paged_blocks(int cus, int head_dim, int requests, int tokens, int count, int kvheads, int group, int length,
                           int window) {
     PagedCut c;
     const int64_t rows = int64_t(count) * group;
+    const int h = head_dim == 32 ? 0 : head_dim == 64 ? 1 : 2;
+    const double row = 2.0 * (head_dim + 4);
+    static const SpanRate kFour[3] = {{4, 4, 5, 1.2, 1.6}, {4, 4, 5, 1.25, 2.4}, {4, 4, 5, 1.85, 4.1}};
+    static const SpanRate kEight[3] = {{8, 8, 5.8, 1.2, 0}, {8, 8, 6, 1.25, 0}, {8, 8, 8, 1.85, 0}};
     const int keys = window > 0 ? static_cast<int>(std::min<int64_t>(length, int64_t(window) + count - 1)) : length;
     // (a grid holds 2^24 blocks of 256 threads)
     const int64_t most = std::max<int64_t>(1, (int64_t(1) << 22) / (int64_t(requests) * kvheads));
     c.small = static_cast<int>(std::min<int64_t>(paged_small(head_dim), most * kSpanRows));
     if (rows <= c.small) {
         c.row_tiles = static_cast<int>((rows + kSpanRows - 1) / kSpanRows);
-        c.rows = cut_span(cus, head_dim, rows, int64_t(requests) * kvheads, keys, keys, 2, false, false);
+        const int64_t pairs = int64_t(requests) * kvheads, tiled = c.row_tiles * pairs;
+        const int tiles = std::max(1, span_tiles(keys) + (window > 0));
+        const double record = double(rows) * pairs * head_dim * 8 / 3e6 + kPiece;
+        best_cut(c.rows, cus, tiled, tiles, keys * row, kFour[h], record, 3.5);
+        best_cut(c.rows, cus, tiled, tiles, keys * row, kEight[h], record, 3.5);
         const int64_t blocks = int64_t(requests) * kvheads * c.row_tiles * c.rows.splits;
         if (by_length(cus, requests, blocks, keys)) c.round = std::max(1, cus / kvheads);
         return c;
@@ -49,10 +63,7 @@ inline PagedCut cut_paged_blocks(int cus, int head_dim, int requests, int tokens
     // Beside blocks of 128, at most four blocks of 16 a request, most of which have no rows (500 decoding requests and a
     // prompt piece, rows of 64 values: eight 112 us, four 96, two 90).
     c.small = std::min(c.small, 64);
-    static const SpanRate kFour[3] = {{4, 4, 5, 1.2, 1.6}, {4, 4, 5, 1.25, 2.4}, {4, 4, 5, 1.85, 4.1}};
     static const SpanRate kWide[3] = {{4, 1, 6, 1.1, 1.27}, {4, 1, 6, 1.25, 1.45}, {4, 1, 6, 1.57, 2.2}};
-    const int h = head_dim == 32 ? 0 : head_dim == 64 ? 1 : 2;
-    const double row = 2.0 * (head_dim + 4);
     // the tokens' whole blocks, and one that is not filled for every request that may have more than `small` rows (every
     // one where they are found without their lengths)
     const int64_t whole = int64_t(tokens) * group / kWideRows, filled = std::max<int64_t>(1, whole);
@@ -65,7 +76,7 @@ inline PagedCut cut_paged_blocks(int cus, int head_dim, int requests, int tokens
         return c;
     }
     c.row_tiles = c.small / kSpanRows;
-    best_cut(c.rows, cus, int64_t(requests) * kvheads, std::max(1, span_tiles(keys)), keys * row, kFour[h], 0.5, 3.5);
+    best_cut(c.rows, cus, int64_t(requests) * kvheads, std::max(1, span_tiles(keys)), keys * row, kFour[h], kPiece, 3.5);
     return c;
 }
 

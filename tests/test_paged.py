@@ -126,6 +126,14 @@ def test_the_tests_of_ordered_requests_reach_the_order(host):
     assert v[8] == 0
 
 
+def test_the_test_of_many_pieces_has_them(host):
+    from tests.test_paged_gpu import MANY_PIECES
+    for hd, past in MANY_PIECES:
+        v = (ct.c_int * 10)()
+        host.cut(hd, 1, 1, 1, 1, 2, past + 1, 0, v)
+        assert v[2] >= 64, (hd, past, v[2])
+
+
 def test_argument_rules(host):
     assert host.pages_rule(1, 10, 16, 2, 64) is None and host.pages_rule(1, 2 ** 27 - 1, 16, 1, 32) is None
     for args, word in [((0, 10, 16, 2, 64), b"positive"), ((1, 0, 16, 2, 64), b"positive"), ((1, 10, 16, 0, 64), b"positive"),

@@ -312,6 +312,20 @@ def test_several_pieces(hd, length):
     b.check(b.run(window=900, length=length), 900)
 
 
+MANY_PIECES = [(32, 66100), (64, 32768), (64, 32767), (128, 16400)]  # rows of so many values, and the longest request's positions
+
+
+@pytest.mark.parametrize("hd,past", MANY_PIECES)
+def test_more_pieces_than_a_wave_has_lanes(hd, past):
+    """One long request by itself and beside short ones, with a length given and cut for the tables' width."""
+    rng = np.random.default_rng(hd + past)
+    b = Batch(rng, 1, 2, hd, [1], [past], page=64)
+    b.check(b.run(length=past + 1))
+    b.check(b.run())
+    b = Batch(rng, 1, 2, hd, [1, 1, 2, 0, 1], [257, -1, past, 4, 0], page=64)
+    b.check(b.run(length=past + 2))
+
+
 ORDERED = [(40, 8), (64, 5), (65, 4), (130, 3), (511, 1)]  # requests and kv heads
 
 

@@ -18,6 +18,8 @@ inline const char *check_pages(int layers, int pages, int page_size, int kvheads
     if (int64_t(kvheads) * page_size * (2 * head_dim + 8) >= (int64_t(1) << 31))
         return "paged cache: the kv heads' rows of a page must be below 2^31 bytes";
     if (int64_t(pages) * page_size >= (int64_t(1) << 31)) return "paged cache: pages * page_size must be below 2^31";
+    if (layers > (int64_t(1) << 46) / (int64_t(pages) * kvheads * page_size * (2 * head_dim + 8)))
+        return "paged cache: more than 2^46 bytes";  // (and the sizes' products would wrap later)
     return nullptr;
 }
 

@@ -140,6 +140,10 @@ def test_argument_rules(host):
                        ((1, 10, 8, 2, 64), b"page_size"), ((1, 10, 24, 2, 64), b"page_size"), ((1, 10, 512, 2, 64), b"page_size"),
                        ((1, 10, 16, 2, 96), b"head_dim"), ((1, 10, 16, 70000, 64), b"65535"), ((1, 10, 256, 40000, 128), b"2^31 bytes"), ((1, 2 ** 27, 16, 2, 64), b"2^31")]:
         assert word in host.pages_rule(*args), args
+    # 2^22 layers of 2^20 pages of over 2^22 bytes: past 2^64, where the sizes wrap
+    assert b"2^46" in host.pages_rule(1 << 22, 1 << 20, 256, 1 << 6, 128)
+    assert b"2^46" in host.pages_rule(2 ** 31 - 1, 2 ** 27 - 1, 16, 65535, 128)
+    assert host.pages_rule(64, 1 << 20, 16, 8, 128) is None
     assert host.requests_rule(0, 1, 16) is None and host.requests_rule(8192, 2 ** 26, 16) is None
     for args, word in [((-1, 1, 16), b"8192"), ((8193, 1, 16), b"8192"), ((1, 0, 16), b"width"), ((1, 2 ** 26 + 1, 16), b"2^30")]:
         assert word in host.requests_rule(*args), args

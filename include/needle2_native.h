@@ -241,7 +241,6 @@ int needle2_gpu_device_info(char *buf, int len);         /* "name;arch;cus;hbm_b
  * what is issued to `stream` between begin and end, instantiate, replay with
  * one launch. Entry points used inside must have run once before the capture
  * and must not read host memory: plan_run, attention (all forms),
- * and must not read host memory: plan_run, attention (all forms),
  * kv_store_device, kv_evict, pages_* (but pages_free) and heads*. */
 int needle2_gpu_graph_begin(void *stream);
 void *needle2_gpu_graph_end(void *stream);                /* instantiated graph, or NULL */
@@ -402,8 +401,9 @@ int needle2_gpu_pages_extend(void *cache, int requests, const int *d_counts, int
 /* Cuts request r to its first keep[r] positions (negative: it stays as it is, and
  * so does one that is not longer; 0: it ends): d_lengths is lowered, and the pages
  * that hold none of them are free again and -1 in d_tables. Right after an
- * extension, a trim to its d_firsts undoes it. Tables that hold pages which another request's table has too, or
- * that no extension dealt, are not for this call. */
+ * extension, a trim to its d_firsts undoes it. Tables that hold pages which
+ * another request's table has too, or that no extension dealt, are not for this
+ * call. */
 int needle2_gpu_pages_trim(void *cache, int requests, const int *d_keep, int *d_lengths, int *d_tables, int width,
                            void *stream);
 /* d_k, d_v: device fp32 rows [tokens], k_stride and v_stride floats from one to

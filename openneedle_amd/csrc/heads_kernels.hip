@@ -5,8 +5,9 @@
 //   y_j sin t) for j < h = rotary / 2, t = position * freq_j;  stored rows as the cache's quantiser has them.
 //
 // t is formed in 64 bits (a position of a million times a frequency in 32 would be off by 0.06), reduced there to an eighth
-// of a turn, and only the rest is rounded: sin and cos are within 2^-23. Everything else is fp32, every result rounded once
-// or twice. A row whose squares pass the fp32 range is normed at 2^-64 of its size.
+// of a turn, and only the rest is rounded: sin and cos are within 2^-23 of t's (which 64 bits hold to 2^-53 of its size).
+// Everything else is fp32, every result rounded once or twice. A row whose squares pass the fp32 range is normed at 2^-64 of
+// its size.
 //
 // Memory bounds many tokens, latency few. A row is one 16-byte piece a lane (HD / 4 lanes); a lane's angles are those of
 // all of a token's rows, so HD / 4 lanes take four of a token's rows, all of them loaded first (8191 tokens, 40 rows of 128

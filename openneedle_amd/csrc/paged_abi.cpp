@@ -170,7 +170,7 @@ static HeadsArgs heads_args(const float *d_q, int q_stride, float *d_q_out, int 
         check_rule(check_rows(d_k, k_stride, kvheads, head_dim));
         if (d_k_out) check_rule(check_rows(d_k_out, k_out_stride, kvheads, head_dim));
     }
-    ND_CHECK((d_q != d_q_out || q_stride == q_out_stride) && (d_k != d_k_out || k_stride == k_out_stride),
+    ND_CHECK((!heads || d_q != d_q_out || q_stride == q_out_stride) && (!kvheads || d_k != d_k_out || k_stride == k_out_stride),
              "heads: rows in place have one stride");
     for (const float *g : {d_q_gain, d_k_gain})
         ND_CHECK(reinterpret_cast<uintptr_t>(g) % 16 == 0, "heads: gains must begin at multiples of 16 bytes");

@@ -7,8 +7,9 @@
 // of `page` writes the table's entry, and a pass over the tokens does all.
 //
 // Latency bounds both kernels: loads, a scan, a search, a page's load and the stores, each after the other (an extension and
-// its trim, 32 requests or 500 with 11000 tokens: 14.6 us). So there is one launch each, in which every block of 1024 tokens scans all requests for itself (16 waves, a request a thread up to 1024 of them), which costs less
-// than a second launch behind the first one's end. Sums saturate instead of growing past 32 bits.
+// its trim, 32 requests or 500 with 11000 tokens: 14.6 us). So there is one launch each, in which every block of 1024 tokens
+// scans all requests for itself (16 waves, a request a thread up to 1024 of them), which costs less than a second launch
+// behind the first one's end. Sums saturate instead of growing past 32 bits.
 #include "paged.h"
 
 namespace nd {

@@ -6,8 +6,8 @@
 //
 // t is formed in 64 bits (a position of a million times a frequency in 32 would be off by 0.06), reduced there to an eighth
 // of a turn, and only the rest is rounded: sin and cos are within 2^-23 of t's (which 64 bits hold to 2^-53 of its size).
-// Everything else is fp32, every result rounded once or twice. A row whose squares pass the fp32 range is normed at 2^-64 of
-// its size.
+// Everything else is fp32, every result rounded once or twice. Where a row's squares pass the fp32 range, or they and eps are
+// so small that the squares lose bits (below 2^-126), the row and eps are taken times a power of two, which is exact.
 //
 // Memory bounds many tokens, latency few. A row is one 16-byte piece a lane (HD / 4 lanes); a lane's angles are those of
 // all of a token's rows, so HD / 4 lanes take four of a token's rows, all of them loaded first (8191 tokens, 40 rows of 128
@@ -48,6 +48,9 @@ __device__ __forceinline__ float group_sum(float v, int t) {
     if constexpr (H < L) return group_sum<L, H * 2>(v + butterfly_partner<H>(v, t), t);
     else return v;
 }
+
+// e of |v| in [2^(e - 1), 2^e); far below every other's for 0.
+__device__ __forceinline__ int exponent(float v) { return v > 0 ? __builtin_amdgcn_frexp_expf(v) : -1000; }
 
 // ROT: 0 none, 1 the whole row (partners half a row apart: HD / 8 lanes), 2 any even number of dimensions (through LDS).
 template <int HD, int ROWS, int ROT>
@@ -95,15 +98,19 @@ __global__ __launch_bounds__(256) void heads_kernel(HeadsArgs a, int parts) {
         float y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
         const float *gain = is_q ? a.q_gain : is_v ? nullptr : a.k_gain;
         if (gain) {
-            float sum = group_sum<L>((y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]), lane);
-            float eps = a.eps;
-            if (__builtin_expect(!(sum < INFINITY), 0)) {
-                eps = 0.0f;  // (below the sum's last bit)
+            auto squares = [&] { return group_sum<L>((y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]), lane); };
+            const float sum = squares();
+            float mean = sum / HD + a.eps;
+            if (__builtin_expect(!(sum < INFINITY && mean >= 0x1p-100f), 0)) {
+                const float top = group_max<L>(fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))), lane);
+                // the row's largest value, or the root of eps where that is larger, to 2^59 .. 2^60: the sum of 128 squares is
+                // below 2^127, and what becomes smaller than a normal number has a result of zero
+                const int up = top < INFINITY ? 60 - max(exponent(top), (exponent(a.eps) + 1) >> 1) : 0;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) y[c] *= 0x1p-64f;
-                sum = group_sum<L>((y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]), lane);
+                for (int c = 0; c < 4; ++c) y[c] = ldexpf(y[c], up);
+                mean = squares() / HD + ldexpf(a.eps, 2 * up);
             }
-            const float r = 1.0f / sqrtf(sum / HD + eps);
+            const float r = 1.0f / sqrtf(mean);
             const float4 g = *reinterpret_cast<const float4 *>(gain + d);
             const float gs[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll

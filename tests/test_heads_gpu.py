@@ -96,6 +96,50 @@ def test_sizes_of_rows(eps):
         assert (np.abs(g - want) <= tol).all()
 
 
+SIZES = [3.3e38, 4.4e37, 1e37, 1e20, 1e19, 1.0, 1e-12, 1e-15, 1e-18, 3e-20, 3e-22, 1e-23, 1e-30, 1e-37, 1e-41]
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("copies", [1, 400])
+@pytest.mark.parametrize("cut", [0, 1, 2])
+@pytest.mark.parametrize("eps", [0.0, 1e-44, 1e-38, 1e-33, 1e-6, 1e29])
+def test_the_norm_over_the_whole_range(hd, copies, cut, eps):
+    """Rows from subnormal values to the largest, whose squares pass the range at either end; rows of one such value among
+    zeros, or beside values of another size; eps from a subnormal number to one far above a row. Scaled by a power of two a
+    row has the errors of any other; only results below the normal numbers are rounded to 2^-149, once before the gain and
+    once after it, and once more when they are rotated."""
+    rng = np.random.default_rng(hd + cut)
+    x = rng.uniform(0.5, 1.0, (len(SIZES), 4, hd)) * rng.choice([-1, 1], (len(SIZES), 4, hd))
+    x[:, 1] = np.sign(x[:, 1])  # values of one size
+    x[:, 2] = 0
+    x[:, 2, hd // 2 + 3] = 1
+    x[:, 3, 1:] *= 2.0 ** -rng.integers(0, 70, hd - 1)
+    x = np.tile((x * np.array(SIZES)[:, None, None]).astype(np.float32), (copies, 1, 1))
+    gain = rng.normal(size=hd).astype(np.float32)
+    freq = rotary_frequencies(1e4, (0, hd, hd - 12)[cut])
+    positions = np.arange(len(x)) % 97
+    eps = float(np.float32(eps))
+    want, tol = heads_of(x, positions, gain, freq, eps)
+    tol = tol + 2.0 ** -149 * (3 + 2 * np.abs(1 + gain.astype(np.float64)).max())
+    for got in run(x, x, positions, gain, gain, freq, eps):
+        assert (np.abs(got - want) <= tol).all()
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-42, 1e-6])
+def test_the_norm_of_zeros(eps):
+    """Zeros where eps is not 0; no number where it is, as the formula has it; the rows beside them as they are."""
+    rng = np.random.default_rng(3)
+    q = rng.normal(size=(5, 3, 64)).astype(np.float32)
+    gain, freq = rng.normal(size=64).astype(np.float32), rotary_frequencies(1e4, 64)
+    clean = run(q, q, np.arange(5), gain, gain, freq, eps)
+    q[1, 2], q[4, 0] = 0, 0
+    for g, c in zip(run(q, q, np.arange(5), gain, gain, freq, eps), clean):
+        for row in (g[1, 2], g[4, 0]):
+            assert np.isnan(row).all() if eps == 0 else not row.any()
+        g[1, 2], g[4, 0] = c[1, 2], c[4, 0]
+        np.testing.assert_array_equal(g, c)
+
+
 def test_rows_of_one_projection_and_tokens_left_out():
     """q and k side by side with v; tokens at negative positions stay as they were; only q, only k; one gain."""
     rng = np.random.default_rng(6)

@@ -134,6 +134,26 @@ def test_the_test_of_many_pieces_has_them(host):
         assert v[2] >= 64, (hd, past, v[2])
 
 
+def test_the_graphs_with_records_have_them(host):
+    """Each captured step has records of both kinds that it can have, every later call more than fit the scratch before it,
+    and the requests of the test have keys for several pieces."""
+    from tests.test_paged_gpu import OUTGROWN, RECORDED as c, RECORDED_COUNTS
+    calls = [(c["tokens"], n) for n in RECORDED_COUNTS] + [(OUTGROWN["tokens"], OUTGROWN["count"])]
+    held_records = held_rows = 0
+    for tokens, count in calls:
+        v = (ct.c_int * 10)()
+        host.cut(c["hd"], c["requests"], tokens, count, c["kvheads"], c["group"], c["width"] * c["page"], 0, v)
+        small, row_tiles, splits, per, _, wide_blocks, wide_splits, wide_per, _, records = v
+        rows = c["requests"] * c["kvheads"] * row_tiles * 16
+        assert splits > 1 and per * 64 < 390  # (keys of the second longest request)
+        if count > 1:
+            rows += tokens * c["kvheads"] * c["group"]
+            assert wide_blocks and wide_splits > 1 and wide_per * 32 < 390 and count * c["group"] > small
+        assert records > held_records and rows > held_rows, (tokens, count)
+        # (the scratch at least doubles)
+        held_records, held_rows = max(records, 2 * held_records), max(rows, 2 * held_rows)
+
+
 def test_argument_rules(host):
     assert host.pages_rule(1, 10, 16, 2, 64) is None and host.pages_rule(1, 2 ** 27 - 1, 16, 1, 32) is None
     for args, word in [((0, 10, 16, 2, 64), b"positive"), ((1, 0, 16, 2, 64), b"positive"), ((1, 10, 16, 0, 64), b"positive"),

@@ -567,6 +567,51 @@ def test_serving_step_captured():
         g.close()
 
 
+RECORDED = dict(hd=64, requests=3, tokens=130, kvheads=2, group=2, width=375, page=16)  # of a captured step
+RECORDED_COUNTS = (1, 130)  # most tokens of a request, in the order in which the steps are captured
+OUTGROWN = dict(tokens=700, count=400)  # of a later eager call
+
+
+def test_graphs_whose_calls_have_records():
+    """Steps cut into pieces, in blocks of 16 rows and of 128, captured in two graphs, each with scratch that the next call
+    outgrows; then they are replayed in turn beside eager calls, which share the larger scratch, every output checked."""
+    rng = np.random.default_rng(24)
+    c, stream = RECORDED, Stream()
+    s = Server(rng, c["requests"], c["tokens"], c["kvheads"] * c["group"], c["kvheads"], c["hd"], 200, c["page"], c["width"], stream)
+    for counts in [[130, 0, 0]] * 6 + [[0, 130, 0]] * 3 + [[0, 0, 5]]:  # stored, not attended
+        rows = s.feed(counts)
+        s.issue(0)
+        synchronize()
+        _, _, slots, positions = s.model.extend(counts, s.tokens)
+        v = rows.reshape(s.tokens, -1, s.hd)[:, s.heads + s.kvheads:]
+        s.rows.put([x if p >= 0 else -1 for x, p in zip(slots, positions)], s.d["k"].to_host(np.float32, (s.tokens, s.kvheads, s.hd)), v)
+    graphs = {}
+    for count, counts in zip(RECORDED_COUNTS, ([1, 1, 1], [3, 60, 1])):
+        s.step(counts, count)
+        s.feed([0] * 3)
+        with Graph.capture(stream) as graphs[count]:
+            s.issue(count)
+
+    def outgrow():
+        b = Batch.__new__(Batch)
+        b.kv, b.rows, b.group, b.tables, b.width = s.kv, s.rows, c["group"], np.array(s.model.tables), s.width
+        b.counts, b.past = [OUTGROWN["count"], 299, 1], [380, 90, 4]
+        b.starts = np.concatenate([[0], np.cumsum(b.counts)])
+        b.q = rng.normal(size=(OUTGROWN["tokens"], s.heads, s.hd)).astype(np.float32)
+        b.check(b.run(length=s.width * s.kv.page_size), rows={(r, i) for r, n in enumerate(b.counts) for i in range(0, n, 37)}, many=True)
+
+    outgrow()
+    for counts, count in (([1, 1, 1], 1), ([70, 1, 2], 130), ([1, 0, 1], 1), ([0, 0, 0], 130), ([1, 1, 0], 1), ([1, 90, 39], 130), ([1, 1, 1], 1)):
+        rows = s.feed(counts)
+        graphs[count].launch(stream)
+        s.verify(counts, rows, count > 8)
+        s.step([1, 0, 2], 2)
+        if count > 8:
+            outgrow()
+    for g in graphs.values():
+        g.close()
+
+
 def test_two_streams_two_caches():
     """Calls of two caches at once, on streams of their own."""
     rng = np.random.default_rng(23)

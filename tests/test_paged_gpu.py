@@ -612,6 +612,31 @@ def test_graphs_whose_calls_have_records():
         g.close()
 
 
+@pytest.mark.parametrize("counts,past", [([1, 0, 2], [20, 40, 10]), ([100, 0, 100], [20, 40, 70])])
+def test_starts_outside_the_batch_are_its_ends(counts, past):
+    """A negative start is the batch's first row, one past its rows their end: the requests between them as ever."""
+    rng = np.random.default_rng(25)
+    b = Batch(rng, 1, 2, 64, counts, past)
+    right = b.starts
+    for first, last in ((-5, 900), (-2 ** 31, 2 ** 31 - 1), (-1, right[-1])):
+        b.starts = np.array([first, right[1], right[2], last])
+        got = b.run()
+        b.starts = right
+        b.check(got, many=max(counts) > 9)
+
+
+@pytest.mark.parametrize("n", [2, 100])
+def test_a_start_behind_the_next_one(n):
+    """Starts that go back: a request whose end lies before its start has no tokens, the others have the rows from their
+    start to their end (a row of two of them is one's or the other's)."""
+    rng = np.random.default_rng(n)
+    b = Batch(rng, 1, 2, 64, [n, 0, n], [20, 40, 10])
+    b.starts = np.array([0, n, n // 2, n // 2 + n])
+    got = b.run()
+    assert np.isnan(got[n // 2 + n:]).all() and np.isfinite(got[:n // 2 + n]).all()
+    b.check(got, rows={(0, i) for i in range(n // 2)} | {(2, i) for i in range(n - n // 2, n)}, many=n > 9)
+
+
 def test_two_streams_two_caches():
     """Calls of two caches at once, on streams of their own."""
     rng = np.random.default_rng(23)

@@ -17,6 +17,7 @@ struct PagedHandle {
     DevBuf<int> stack, state;  // state: free pages; blocks of a running launch that are done
     KeptBuf<float> records;    // of the attention (span.h)
     KeptBuf<int2> some;
+    const int2 *zeroed = nullptr;  // the last of `some`, once zeros have been written to it and not only captured
 
     size_t layer_bytes() const { return size_t(pages) * kvheads * page_block_bytes(shift, head_dim); }
     PageStack free() const { return PageStack{stack.p, state.p, state.p + 1, pages}; }
@@ -280,10 +281,14 @@ int needle2_gpu_pages_attention(void *h, int layer, const float *d_q, float *d_o
             a.wide_o = a.rec_o + n * p.head_dim;
             a.rec_ml = reinterpret_cast<float2 *>(a.wide_o + m * p.head_dim);
             a.wide_ml = a.rec_ml + n;
-            const int2 *before = p.some.bufs.empty() ? nullptr : p.some.bufs.back()->p;
             a.some = p.some.reserve(few + many);
             a.wide_some = a.some + few;
-            if (a.some != before) launch_zero(a.some, p.some.bufs.back()->n, s);
+            if (a.some != p.zeroed) {
+                launch_zero(a.some, p.some.bufs.back()->n, s);
+                hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+                ND_HIP(hipStreamIsCapturing(s, &capture));
+                if (capture == hipStreamCaptureStatusNone) p.zeroed = a.some;
+            }
         }
         launch_paged(a, p.head_dim, s);
         if (few) launch_paged_join(a, int64_t(few), p.head_dim, s);

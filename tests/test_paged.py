@@ -139,6 +139,10 @@ def test_the_graphs_with_records_have_them(host):
     and the requests of the test have keys for several pieces."""
     from tests.test_paged_gpu import OUTGROWN, RECORDED as c, RECORDED_COUNTS
     calls = [(c["tokens"], n) for n in RECORDED_COUNTS] + [(OUTGROWN["tokens"], OUTGROWN["count"])]
+    for counts in ((1, 1), (130, 1)):  # and those of a first call that is captured
+        v = (ct.c_int * 10)()
+        host.cut(64, 2, sum(counts), max(counts), 2, 2, 3001, 0, v)
+        assert v[9] > 0 and v[2] > 1 and v[3] * 64 < 900 and (max(counts) == 1 or (v[6] > 1 and v[7] * 32 < 1200))
     held_records = held_rows = 0
     for tokens, count in calls:
         v = (ct.c_int * 10)()

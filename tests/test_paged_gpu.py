@@ -2,6 +2,8 @@
 tokens against the closed form in 64 bits with the tolerance of tests/test_span_gpu.py (many rows over the same keys: as
 check_many_rows there, tiles of 32 positions), and a whole serving step, eager and captured.
 """
+import ctypes as ct
+
 import numpy as np
 import pytest
 
@@ -609,6 +611,39 @@ def test_graphs_whose_calls_have_records():
         if count > 8:
             outgrow()
     for g in graphs.values():
+        g.close()
+
+
+def test_a_capture_that_grows_the_scratch_comes_first():
+    """A first call captured in a relaxed capture, which may allocate: what it captures has not run when the same call is
+    made eagerly, before the graph's first replay and after it."""
+    rng = np.random.default_rng(26)
+    stream, lib = Stream(), _ffi.lib()
+    for counts, past in (([1, 1], [3000, 900]), ([130, 1], [1200, 900])):
+        b = Batch(rng, 2, 2, 64, counts, past)
+        held = [upload(b.q), ints(b.starts), ints(b.past), ints(b.tables)]
+        out = DeviceArray.from_host(np.full(b.q.shape, np.nan, np.float32))
+
+        def call():
+            b.kv.attention(0, held[0], out, 4, 2, len(b.q), max(counts), *held[1:], b.width, 3001, stream=stream)
+
+        rows = {(r, i) for r, n in enumerate(counts) for i in range(0, n, 13)}
+        assert lib.hipStreamBeginCapture(ct.c_void_p(stream.ptr), 2) == 0
+        try:
+            call()
+        finally:
+            g = Graph()
+            g.ptr = lib.needle2_gpu_graph_end(stream.ptr)
+        assert g.ptr
+        for replay in (False, True, True, False):
+            out.fill(0xFF)
+            synchronize()
+            if replay:
+                g.launch(stream)
+            else:
+                call()
+            synchronize()
+            b.check(out.to_host(np.float32, b.q.shape), rows=rows, many=max(counts) > 9)
         g.close()
 
 

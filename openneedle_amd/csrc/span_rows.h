@@ -177,7 +177,7 @@ __device__ __forceinline__ void span_rows(const A &a, int bx, int kh, int unit) 
             const auto rv = rv_of(i);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const uint32_t at = vb + i * step + u * HD;
+                const uint32_t at = vb + (PAGED ? u : 16 * i + u) * HD;  // (one constant: an instruction's own offset)
                 if constexpr (VB == 8) {
                     const auto w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, at, 0, 0));
                     T.v[i][u][0] = w.x;

@@ -415,7 +415,8 @@ int needle2_gpu_pages_store(void *cache, int layer, const float *d_k, int k_stri
 /* Norms and rotation of the heads of q and k, as in Engine::step
  * (needle2/csrc/engine.cpp:994-1004) for a batch of tokens: where a gain
  * ([head_dim], nullable: not normed) is set, a head x becomes
- * x / sqrt(mean(x^2) + eps) * (1 + gain); then dimensions j and j + rotary / 2 are
+ * x / sqrt(mean(x^2) + eps) * (1 + gain), for x and eps of any size (zeros with eps 0
+ * are no number); then dimensions j and j + rotary / 2 are
  * turned by d_positions[token] * d_freq[j] (device fp64 [rotary / 2]; rotary 0:
  * not at all). head_dim 32, 64 or 128. Rows as in pages_store, of heads * head_dim
  * and kvheads * head_dim (0: none); outputs in place (with the same stride) or in
@@ -440,9 +441,14 @@ int needle2_gpu_heads_store(void *cache, int layer, const float *d_q, int q_stri
  * negative first position, or whose tokens pass its table, yields zeros; positions
  * of no page are not attended. Rows of no request are left as they were. heads: a
  * multiple of kvheads, 1 to 16 per kv head; at most 2^25 query rows. length: the
- * most positions that a request has (0: unknown): how the work is cut goes by it,
- * the results do not depend on it. Exactness, and heads without a softmax, as
- * described above for long contexts. */
+ * most positions that a request has (0: unknown; a wrong one costs time only). How the
+ * work is cut goes by it, and by requests, tokens and count: a request's outputs have
+ * the same exactness for any of them, but not the same bits, since sums are added in
+ * another order (the same call gives the same bits). requests, tokens and count are
+ * bounds; where count tokens may be more than 192 rows of 32 values (128 of 64, 64 of
+ * 128; tokens times heads per kv head), those of more than 512 requests cost time for
+ * requests that do not come.
+ * Exactness, and heads without a softmax, as described above for long contexts. */
 int needle2_gpu_pages_attention(void *cache, int layer, const float *d_q, float *d_out, int heads, int requests, int tokens,
                                 int count, const int *d_starts, const int *d_firsts, const int *d_tables, int width,
                                 int length, int window, void *stream);

@@ -12,7 +12,9 @@
 // Memory bounds many tokens, latency few. A row is one 16-byte piece a lane (HD / 4 lanes); a lane's angles are those of
 // all of a token's rows, so HD / 4 lanes take four of a token's rows, all of them loaded first (8191 tokens, 40 rows of 128
 // values: 66.4 us, 5.05 TB/s; with two or eight rows 72.7 and 69.9), and two where nothing is rotated (8191 tokens' K and V
-// rows of 8 heads of 128 into slots: 19.7 us, 4.3 TB/s; four or eight rows 20.6 and 21.9).
+// rows of 8 heads of 128 into slots: 19.7 us, 4.3 TB/s; four or eight rows 20.6 and 21.9). Half of each of the 40 rows
+// rotated, through LDS: 70 us; 32 rows of q, 8 of k and 8 of v, those of k and v into slots: 74.4, 4.7 TB/s, and 79 with half
+// of each rotated (in a graph, where the 40 whole rows take 64).
 #include "paged.h"
 #include "span_dev.h"
 

@@ -28,7 +28,8 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_kernel(PagedSpanArgs a) {
     paged_rows<HD, NW>(a, blockIdx.x);
 }
 
-// The blocks of 128 rows first: they take the longest.
+// The blocks of 128 rows first: they take the longest. With rows of 128 values 23 registers a lane are kept in memory, one of
+// them read in the loop over tiles.
 template <int HD>
 __global__ __launch_bounds__(256, 2) void paged_wide_kernel(PagedSpanArgs a, int blocks) {
     if (static_cast<int>(blockIdx.x) < blocks) span_wide<HD, Keys::Paged>(a, blockIdx.x);

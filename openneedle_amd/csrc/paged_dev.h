@@ -52,8 +52,12 @@ __device__ __forceinline__ WideBlock wide_block(const PagedSpanArgs &a, int b, i
 
 // The same for at most kRanked requests, those in blocks of 128 rows by the length of their keys, the longest first, and of
 // each the last row tile, which attends the most, first: what takes longest does not begin last, and no block has a request
-// of fewer rows (rows of 64 values: 20 pieces of up to 300 tokens 306 -> 266 us, two of up to 800 beside 200 decoding
-// requests 176 -> 106; of 128: three beside 48 as before, 252 us). row -1: there is no such block.
+// of fewer rows. In wide_block's order and this one (contexts of 4000): 20 pieces of up to 300 tokens, rows of 64 values, 8
+// kv heads of 4 heads 358 and 341 us, 4 of 2 171 and 179; two of up to 800 beside 200 decoding requests 185 and 187, 107
+// and 107; three of up to 1024 beside 48, rows of 128, 256 and 256, 129 and 129. But every block looks at every request
+// that is in blocks of 128, one after the other: of up to 8 tokens with 16 heads (rows of 128, 4 kv heads, contexts of 1000)
+// 64, 128, 256, 512 requests 61, 78, 150, 271 us in wide_block's and 68, 98, 260, 775 in this. row -1: there is no such
+// block.
 __device__ __forceinline__ WideBlock ranked_block(const PagedSpanArgs &a, int b, int lane) {
     constexpr int kEach = kRanked / 64;
     const ND_GLOBAL int *starts = (const ND_GLOBAL int *)(a.starts), *firsts = (const ND_GLOBAL int *)(a.positions);

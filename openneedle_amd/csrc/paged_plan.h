@@ -34,7 +34,7 @@ struct PagedCut {
 // us that one piece more costs blocks of 16 rows (one request of 60000 positions, rows of 32 values: 32, 64 and 118 pieces
 // 20.2, 17.7 and 17.0 us). At span_plan.h's 0.5 requests were cut too coarsely: one of 1500, 8000 and 30000 positions, rows
 // of 64, took 13.1, 14.6 and 20.9 us and takes 10.5, 11.6 and 17.4; one of 4000, rows of 128, 16.4 and 13.3; but twelve of
-// 600 there 14.1 and 15.3.
+// 600 there 14.1 and 15.3: one price for all of them, which gives these up for the others.
 constexpr double kPiece = 0.03;
 
 inline PagedCut cut_paged_blocks(int cus, int head_dim, int requests, int tokens, int count, int kvheads, int group, int length,
@@ -61,11 +61,14 @@ inline PagedCut cut_paged_blocks(int cus, int head_dim, int requests, int tokens
         return c;
     }
     // Beside blocks of 128, at most four blocks of 16 a request, most of which have no rows (500 decoding requests and a
-    // prompt piece, rows of 64 values: eight 112 us, four 96, two 90).
+    // prompt piece, rows of 64 values: eight 112 us, four 96, two 90). With two, requests of 33 to 64 rows would be in blocks
+    // of 128: 20, 100 and 250 requests of 36 to 48 rows beside a piece of 600 tokens, rows of 64, 48, 79, 130 us with four
+    // and 65, 125, 248 with two; of 128 73, 114, 231 and 91, 160, 310.
     c.small = std::min(c.small, 64);
     static const SpanRate kWide[3] = {{4, 1, 6, 1.1, 1.27}, {4, 1, 6, 1.25, 1.45}, {4, 1, 6, 1.57, 2.2}};
     // the tokens' whole blocks, and one that is not filled for every request that may have more than `small` rows (every
-    // one where they are found without their lengths)
+    // one where they are found without their lengths, which costs: a piece of 300 tokens, rows of 64, 4 kv heads, contexts of
+    // 4096, under a bound of 1, 512, 513, 2048, 8192 requests 27, 35, 113, 406, 1866 us)
     const int64_t whole = int64_t(tokens) * group / kWideRows, filled = std::max<int64_t>(1, whole);
     c.wide_blocks = static_cast<int>(whole + (requests > kRanked ? requests
                                                                  : std::min<int64_t>(requests, int64_t(tokens) * group / (c.small + 1) + 1)));

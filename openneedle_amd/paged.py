@@ -86,7 +86,8 @@ class PagedCache:
         ``r`` has rows ``d_starts[r] .. d_starts[r + 1] - 1``, at most ``count`` of them, the first at position
         ``d_firsts[r]`` (negative: zeros); a token attends its request's positions up to its own, the last ``window`` of
         them if that is not 0. ``length``: the most positions of a request (0: unknown), by which only the cut of the
-        work goes. Rows of no request are left as they were."""
+        work goes: results for another one, or beside other requests, agree within the attention's exactness, not bit
+        for bit. Rows of no request are left as they were."""
         check(self._lib.needle2_gpu_pages_attention(self.ptr, layer, addr(d_q), addr(d_out), int(heads), int(requests),
                                                     int(tokens), int(count), addr(d_starts), addr(d_firsts),
                                                     addr(d_tables), int(width), int(length), int(window),
